@@ -53,6 +53,7 @@ void check_status(int rc, const char* what) {
 }  // namespace
 
 void register_linalg_ops(pybind11::module& m);  // torch_ext_linalg.cpp
+void register_layer_ops(pybind11::module& m);   // torch_ext_layer.cpp
 
 void decode_codebook(int64_t cb, at::Tensor out_lut) {
   TORCH_CHECK(cb >= 0 && cb <= 2, "cb must be 0, 1, or 2");
@@ -303,4 +304,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("pack_trellis", &pack_trellis, py::arg("states"), py::arg("packed"), py::arg("K"),
         "Pack 16-bit trellis states into the EXL3 container (SWAP16 storage)");
   register_linalg_ops(m);
+  register_layer_ops(m);
 }

@@ -1,0 +1,347 @@
+// PyTorch binding of the layer operators (rotary positions, block norms,
+// gated delta rule). Wrong shapes and types raise ValueError; outputs and
+// workspaces come from the caching allocator on the current stream.
+#include <ATen/MemoryOverlap.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include <tuple>
+
+#include "../../include/exl3k.h"
+
+namespace {
+
+using OptTensor = c10::optional<at::Tensor>;
+
+exl3_stream_t cur_stream(const at::Tensor& t) {
+  return reinterpret_cast<exl3_stream_t>(at::cuda::getCurrentCUDAStream(t.device().index()).stream());
+}
+
+void check_rc(int rc, const char* what) {
+  TORCH_CHECK(rc == 0, what, " failed (status ", rc, "): ", exl3_last_error());
+}
+
+int dtype_code(const at::Tensor& t, const char* name, bool f32) {
+  if (t.scalar_type() == at::kHalf) return EXL3_F16;
+  if (t.scalar_type() == at::kBFloat16) return EXL3_BF16;
+  TORCH_CHECK_VALUE(f32 && t.scalar_type() == at::kFloat, name, " must be float16", f32 ? ", " : " or ",
+                    "bfloat16", f32 ? " or float32" : "", ", got ", t.scalar_type());
+  return EXL3_F32;
+}
+
+void check_like(const at::Tensor& t, const at::Tensor& ref, const char* name, const char* ref_name) {
+  TORCH_CHECK_VALUE(t.device() == ref.device(), name, " must be on ", ref.device(), " like ", ref_name,
+                    ", got ", t.device());
+  TORCH_CHECK_VALUE(t.scalar_type() == ref.scalar_type(), name, " must be ", ref.scalar_type(), " like ",
+                    ref_name, ", got ", t.scalar_type());
+}
+
+// The operators have no backward: a graph through them would lose its
+// gradient without a word.
+void check_no_grad(std::initializer_list<const at::Tensor*> ts, const char* what) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const at::Tensor* t : ts)
+    TORCH_CHECK(!t || !t->defined() || !t->requires_grad(), what,
+                " computes no gradient: call it under torch.no_grad()");
+}
+
+const at::Tensor* ptr(const OptTensor& t) { return t.has_value() && t->defined() ? &*t : nullptr; }
+
+// The last dimension contiguous, as the kernels read it; else a copy.
+at::Tensor inner_contiguous(const at::Tensor& t) {
+  return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+
+void fill_rotary(const at::Tensor& t, bool heads_first, int64_t (&st)[3]) {
+  st[0] = t.stride(0);
+  st[1] = t.stride(heads_first ? 2 : 1);
+  st[2] = t.stride(heads_first ? 1 : 2);
+}
+
+// An output of x's shape: of its memory layout where that is dense, so that a
+// transposed view stays one
+at::Tensor out_like(const at::Tensor& x) { return at::empty_like(x); }
+
+}  // namespace
+
+std::tuple<at::Tensor, OptTensor> apply_rotary(at::Tensor q, OptTensor k_opt, at::Tensor positions,
+                                               at::Tensor inv_freq, double factor, bool interleaved,
+                                               bool heads_first, bool transposed, bool inplace) {
+  const at::Tensor* kp = ptr(k_opt);
+  TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
+  TORCH_CHECK_VALUE(q.dim() == 3 || q.dim() == 4, "q must be (tokens, heads, dim) or 4-D, got ", q.dim(), "-D");
+  check_no_grad({&q, kp, &inv_freq}, "apply_rotary");
+  const bool flat = q.dim() == 3;
+  exl3_rotary_args a = {};
+  a.dtype = dtype_code(q, "q", true);
+  if (inplace) {
+    TORCH_CHECK_VALUE(q.stride(-1) == 1 && (!kp || kp->stride(-1) == 1),
+                      "an in-place rotation needs contiguous head elements");
+    at::assert_no_internal_overlap(q);
+    if (kp) at::assert_no_internal_overlap(*kp);
+  }
+  at::Tensor q4 = inner_contiguous(flat ? q.unsqueeze(0) : q), k4;
+  const int tok = heads_first ? 2 : 1, hd = heads_first ? 1 : 2;
+  a.batch = q4.size(0);
+  a.tokens = q4.size(tok);
+  a.q_heads = (int)q4.size(hd);
+  a.dim = (int)q4.size(3);
+  if (kp) {
+    check_like(*kp, q, "k", "q");
+    TORCH_CHECK_VALUE(kp->dim() == q.dim(), "k must have as many dimensions as q");
+    k4 = inner_contiguous(flat ? kp->unsqueeze(0) : *kp);
+    TORCH_CHECK_VALUE(k4.size(0) == a.batch && k4.size(tok) == a.tokens && k4.size(3) == a.dim,
+                      "k must have q's batch, tokens and head size");
+    a.k_heads = (int)k4.size(hd);
+  }
+  TORCH_CHECK_VALUE(a.q_heads >= 1 && a.dim >= 2, "q must have heads of at least two elements");
+  TORCH_CHECK_VALUE(positions.device() == q.device(), "positions must be on ", q.device());
+  TORCH_CHECK_VALUE(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong,
+                    "positions must be int32 or int64, got ", positions.scalar_type());
+  TORCH_CHECK_VALUE((positions.dim() == 1 && positions.size(0) == a.tokens) ||
+                        (positions.dim() == 2 && !flat && positions.size(1) == a.tokens &&
+                         (positions.size(0) == a.batch || positions.size(0) == 1)),
+                    "positions must be (tokens) or (batch, tokens) = (", a.batch, ", ", a.tokens, ")");
+  TORCH_CHECK_VALUE(inv_freq.device() == q.device() && inv_freq.scalar_type() == at::kFloat &&
+                        inv_freq.dim() == 1 && inv_freq.is_contiguous(),
+                    "inv_freq must be a contiguous 1-D float32 tensor on ", q.device());
+  a.rotary_dim = (int)(2 * inv_freq.numel());
+  TORCH_CHECK_VALUE(a.rotary_dim >= 2 && a.rotary_dim <= a.dim && a.dim <= 8192, "inv_freq has ",
+                    inv_freq.numel(), " frequencies for heads of ", a.dim, " elements");
+  a.position_strides[0] = positions.dim() == 2 && positions.size(0) > 1 ? positions.stride(0) : 0;
+  a.position_strides[1] = positions.stride(-1);
+  a.positions_64 = positions.scalar_type() == at::kLong;
+  a.interleaved = interleaved;
+  a.transposed = transposed;
+  a.factor = (float)factor;
+  c10::cuda::CUDAGuard g(q.device());
+  at::Tensor qo = inplace ? q4 : out_like(q4), ko;
+  fill_rotary(q4, heads_first, a.q_strides);
+  fill_rotary(qo, heads_first, a.q_out_strides);
+  if (kp) {
+    ko = inplace ? k4 : out_like(k4);
+    fill_rotary(k4, heads_first, a.k_strides);
+    fill_rotary(ko, heads_first, a.k_out_strides);
+    a.k = k4.data_ptr();
+    a.k_out = ko.data_ptr();
+  }
+  a.q = q4.data_ptr();
+  a.q_out = qo.data_ptr();
+  a.positions = positions.data_ptr();
+  a.inv_freq = inv_freq.data_ptr<float>();
+  check_rc(exl3_rotary(&a, cur_stream(q)), "apply_rotary");
+  if (flat) {
+    qo = qo.squeeze(0);
+    if (kp) ko = ko.squeeze(0);
+  }
+  return {qo, kp ? OptTensor(ko) : OptTensor()};
+}
+
+std::tuple<at::Tensor, OptTensor> block_norm(at::Tensor x, OptTensor weight, OptTensor gate,
+                                             int64_t gate_activation, OptTensor residual,
+                                             double residual_scale, OptTensor scale,
+                                             OptTensor next_weight, double eps, double weight_offset) {
+  TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "x must have at least one element per row");
+  const at::Tensor *w = ptr(weight), *z = ptr(gate), *res = ptr(residual), *sc = ptr(scale),
+                   *nw = ptr(next_weight);
+  check_no_grad({&x, w, z, res, sc, nw}, "block_norm");
+  TORCH_CHECK_VALUE(w || z || res || nw, "nothing to do: give a weight, a gate, a residual or a next_weight");
+  TORCH_CHECK_VALUE(!sc || res, "a scale needs a residual");
+  exl3_block_norm_args a = {};
+  a.dtype = dtype_code(x, "x", true);
+  a.param_dtype = a.dtype;
+  a.d = x.size(-1);
+  a.rows = x.numel() / a.d;
+  const at::Tensor* first = nullptr;
+  for (auto [p, name] : {std::pair<const at::Tensor*, const char*>{w, "weight"}, {nw, "next_weight"}, {sc, "scale"}}) {
+    if (!p) continue;
+    TORCH_CHECK_VALUE(p->device() == x.device(), name, " must be on ", x.device());
+    TORCH_CHECK_VALUE(p->dim() == 1 && p->size(0) == a.d && p->is_contiguous(), name,
+                      " must be a contiguous vector of ", a.d, " elements");
+    TORCH_CHECK_VALUE(p->scalar_type() == x.scalar_type() || p->scalar_type() == at::kFloat, name,
+                      " must be ", x.scalar_type(), " or float32, got ", p->scalar_type());
+    TORCH_CHECK_VALUE(!first || p->scalar_type() == first->scalar_type(),
+                      "weight, next_weight and scale must have one type");
+    first = p;
+    if (p->scalar_type() == at::kFloat) a.param_dtype = EXL3_F32;
+  }
+  for (auto [p, name] : {std::pair<const at::Tensor*, const char*>{z, "gate"}, {res, "residual"}}) {
+    if (!p) continue;
+    check_like(*p, x, name, "x");
+    TORCH_CHECK_VALUE(p->sizes() == x.sizes(), name, " must have x's shape");
+  }
+  c10::cuda::CUDAGuard g(x.device());
+  // rows of one stride: a view that has them is read in place
+  const auto rows = [&](const at::Tensor& t, int64_t& stride) {
+    at::Tensor r = t.dim() == 2 && t.stride(1) == 1 ? t : t.reshape({a.rows, a.d});
+    if (a.d > 1 && r.stride(1) != 1) r = r.contiguous();
+    stride = r.stride(0);
+    return r;
+  };
+  const at::Tensor xr = rows(x, a.x_stride);
+  at::Tensor zr, rr, hidden, normed;
+  a.x = xr.data_ptr();
+  if (z) {
+    zr = rows(*z, a.gate_stride);
+    a.gate = zr.data_ptr();
+    a.gate_activation = (int)gate_activation;
+  }
+  if (res) {
+    rr = rows(*res, a.residual_stride);
+    a.residual = rr.data_ptr();
+  }
+  if (w || z || res) {
+    hidden = at::empty(x.sizes(), x.options());
+    a.hidden = hidden.data_ptr();
+    a.hidden_stride = a.d;
+  } else {
+    hidden = x;
+  }
+  if (nw) {
+    normed = at::empty(x.sizes(), x.options());
+    a.normed = normed.data_ptr();
+    a.normed_stride = a.d;
+    a.next_weight = nw->data_ptr();
+  }
+  a.weight = w ? w->data_ptr() : nullptr;
+  a.scale = sc ? sc->data_ptr() : nullptr;
+  a.eps = (float)eps;
+  a.weight_offset = (float)weight_offset;
+  a.residual_scale = (float)residual_scale;
+  check_rc(exl3_block_norm(&a, cur_stream(x)), "block_norm");
+  return {hidden, nw ? OptTensor(normed) : OptTensor()};
+}
+
+namespace {
+
+// q, k (tokens, key_heads, dk), v (tokens, heads, dv), g and beta (tokens,
+// heads). The tensors that `a` points into are left in the references.
+void fill_delta(exl3_delta_args& a, at::Tensor& q, at::Tensor& k, at::Tensor& v, at::Tensor& g,
+                at::Tensor& beta, double scale, bool normalize_qk, const char* what) {
+  TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
+  check_no_grad({&q, &k, &v, &g, &beta}, what);
+  TORCH_CHECK_VALUE(q.dim() == 3 && k.dim() == 3 && v.dim() == 3, "q, k and v must be (tokens, heads, dim)");
+  check_like(k, q, "k", "q");
+  check_like(v, q, "v", "q");
+  a.dtype = dtype_code(q, "q", false);
+  a.tokens = q.size(0);
+  a.key_heads = (int)q.size(1);
+  a.dk = (int)q.size(2);
+  a.heads = (int)v.size(1);
+  a.dv = (int)v.size(2);
+  TORCH_CHECK_VALUE(k.sizes() == q.sizes(), "k must have q's shape");
+  TORCH_CHECK_VALUE(v.size(0) == a.tokens, "v must have q's ", a.tokens, " tokens");
+  TORCH_CHECK_VALUE(a.key_heads >= 1 && a.heads >= 1 && a.heads % a.key_heads == 0, "value heads (", a.heads,
+                    ") must be a positive multiple of the key heads (", a.key_heads, ")");
+  TORCH_CHECK_VALUE(a.dk >= 8 && a.dk <= 256 && a.dk % 8 == 0, "dk must be a multiple of 8 up to 256, got ", a.dk);
+  TORCH_CHECK_VALUE(a.dv >= 8 && a.dv <= 65536 && a.dv % 8 == 0, "dv must be a positive multiple of 8, got ", a.dv);
+  for (auto [p, name] : {std::pair<at::Tensor*, const char*>{&g, "g"}, {&beta, "beta"}}) {
+    TORCH_CHECK_VALUE(p->device() == q.device(), name, " must be on ", q.device());
+    TORCH_CHECK_VALUE(p->scalar_type() == at::kFloat, name, " must be float32, got ", p->scalar_type());
+    TORCH_CHECK_VALUE(p->dim() == 2 && p->size(0) == a.tokens && p->size(1) == a.heads, name,
+                      " must be (tokens, heads) = (", a.tokens, ", ", a.heads, ")");
+    *p = inner_contiguous(*p);
+  }
+  q = inner_contiguous(q);
+  k = inner_contiguous(k);
+  v = inner_contiguous(v);
+  for (int i = 0; i < 2; ++i) {
+    a.q_strides[i] = q.stride(i);
+    a.k_strides[i] = k.stride(i);
+    a.v_strides[i] = v.stride(i);
+  }
+  a.g_stride = g.stride(0);
+  a.beta_stride = beta.stride(0);
+  a.q = q.data_ptr();
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.g = g.data_ptr<float>();
+  a.beta = beta.data_ptr<float>();
+  a.scale = (float)scale;
+  a.normalize_qk = normalize_qk;
+}
+
+void check_state(const at::Tensor& s, const at::Tensor& q, const exl3_delta_args& a, const char* name) {
+  TORCH_CHECK_VALUE(s.device() == q.device() && s.scalar_type() == at::kFloat, name,
+                    " must be a float32 tensor on ", q.device());
+  TORCH_CHECK_VALUE(s.dim() == 4 && s.size(1) == a.heads && s.size(2) == a.dk && s.size(3) == a.dv, name,
+                    " must be (*, ", a.heads, ", ", a.dk, ", ", a.dv, "), got ", s.sizes());
+}
+
+}  // namespace
+
+at::Tensor gated_delta_step_(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor g, at::Tensor beta,
+                             at::Tensor state, OptTensor slots, double scale, bool normalize_qk) {
+  exl3_delta_args a = {};
+  c10::cuda::OptionalCUDAGuard guard;
+  if (q.is_cuda()) guard.set_device(q.device());
+  fill_delta(a, q, k, v, g, beta, scale, normalize_qk, "gated_delta_step_");
+  check_state(state, q, a, "state");
+  check_no_grad({&state}, "gated_delta_step_");
+  TORCH_CHECK_VALUE(state.is_contiguous() && reinterpret_cast<uintptr_t>(state.data_ptr()) % 16 == 0,
+                    "state must be contiguous and 16-byte aligned (it is updated in place)");
+  a.seqs = a.tokens;
+  a.num_slots = state.size(0);
+  if (const at::Tensor* sl = ptr(slots)) {
+    TORCH_CHECK_VALUE(sl->device() == q.device() && sl->scalar_type() == at::kInt && sl->dim() == 1 &&
+                          sl->size(0) == a.tokens && sl->is_contiguous(),
+                      "slots must be a contiguous int32 vector of ", a.tokens, " elements on ", q.device());
+    a.slots = sl->data_ptr<int32_t>();
+    TORCH_CHECK_VALUE(a.num_slots >= 1 || a.tokens == 0, "state has no slots");
+  } else {
+    TORCH_CHECK_VALUE(a.num_slots == a.tokens, "state must hold one state per token (", a.tokens, "), got ",
+                      a.num_slots);
+  }
+  at::Tensor out = at::empty({a.tokens, a.heads, a.dv}, q.options());
+  if (a.tokens == 0) return out;
+  a.out = out.data_ptr();
+  a.state_out = state.data_ptr<float>();
+  check_rc(exl3_delta_step(&a, cur_stream(q)), "gated_delta_step_");
+  return out;
+}
+
+std::tuple<at::Tensor, at::Tensor> gated_delta_rule(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor g,
+                                                    at::Tensor beta, at::Tensor cu_seqlens,
+                                                    OptTensor initial_state, double scale,
+                                                    bool normalize_qk) {
+  exl3_delta_args a = {};
+  c10::cuda::OptionalCUDAGuard guard;
+  if (q.is_cuda()) guard.set_device(q.device());
+  fill_delta(a, q, k, v, g, beta, scale, normalize_qk, "gated_delta_rule");
+  TORCH_CHECK_VALUE(cu_seqlens.device() == q.device() && cu_seqlens.scalar_type() == at::kInt &&
+                        cu_seqlens.dim() == 1 && cu_seqlens.size(0) >= 1 && cu_seqlens.is_contiguous(),
+                    "cu_seqlens must be a contiguous int32 vector on ", q.device());
+  TORCH_CHECK_VALUE(a.tokens < (1ll << 31), "too many tokens for int32 offsets");
+  a.seqs = cu_seqlens.size(0) - 1;
+  a.cu_seqlens = cu_seqlens.data_ptr<int32_t>();
+  at::Tensor s0;
+  if (const at::Tensor* p = ptr(initial_state)) {
+    check_state(*p, q, a, "initial_state");
+    check_no_grad({p}, "gated_delta_rule");
+    TORCH_CHECK_VALUE(p->size(0) == a.seqs, "initial_state must hold ", a.seqs, " states, got ", p->size(0));
+    s0 = p->contiguous();
+    if (reinterpret_cast<uintptr_t>(s0.data_ptr()) % 16) s0 = s0.clone();
+    a.state_in = s0.data_ptr<float>();
+  }
+  at::Tensor out = at::empty({a.tokens, a.heads, a.dv}, q.options());
+  at::Tensor state = at::empty({a.seqs, a.heads, a.dk, a.dv}, q.options().dtype(at::kFloat));
+  if (a.seqs == 0) return {out.zero_(), state};
+  a.out = out.data_ptr();
+  a.state_out = state.data_ptr<float>();
+  const size_t bytes = exl3_delta_rule_ws_bytes(&a);
+  TORCH_CHECK(bytes > 0, "gated_delta_rule: ", exl3_last_error());
+  at::Tensor ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+  check_rc(exl3_delta_rule(&a, ws.data_ptr(), bytes, cur_stream(q)), "gated_delta_rule");
+  return {out, state};
+}
+
+void register_layer_ops(pybind11::module& m) {
+  m.def("apply_rotary", &apply_rotary, "Rotary positions on q and k (rotary.apply_rotary)");
+  m.def("block_norm", &block_norm, "Norms around a block with gate and residual (norms.block_norm)");
+  m.def("gated_delta_step_", &gated_delta_step_,
+        "One token of the gated delta rule, states in place (delta_rule.gated_delta_step_)");
+  m.def("gated_delta_rule", &gated_delta_rule,
+        "The gated delta rule over packed sequences (delta_rule.gated_delta_rule)");
+}

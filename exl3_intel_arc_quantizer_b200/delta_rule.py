@@ -1,0 +1,89 @@
+"""The gated delta rule on B200: the recurrence of a gated linear-attention
+layer (the ``linear_attn.*`` projections of ``calibration.hessian_groups``),
+over whole sequences (``exl3_delta_rule``) and for one token at a time
+(``exl3_delta_step``).
+
+Per value head, with the state S (dk, dv) in fp32::
+
+    S_t = e^{g_t} S_{t-1} + k_t u_t^T,   u_t = beta_t (v_t - e^{g_t} S_{t-1}^T k_t)
+    o_t = scale S_t^T q_t
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from ._ext import ext, require_cuda
+
+
+def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor,
+                     beta: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None,
+                     initial_state: Optional[torch.Tensor] = None,
+                     scale: Optional[float] = None, normalize_qk: bool = False
+                     ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Outputs and final states, ``(o, state)``, of whole sequences.
+
+    Packed: ``q`` and ``k`` (tokens, key_heads, dk), ``v`` (tokens, heads,
+    dv), ``g`` and ``beta`` (tokens, heads); sequence s is the tokens
+    ``cu_seqlens[s] .. cu_seqlens[s + 1]`` (int32, on the device, never read
+    by the host, not decreasing; lengths of zero are fine; outputs of tokens
+    before the first and after the last sequence are zero). Without
+    ``cu_seqlens`` the tokens are one sequence, or, with a batch dimension in
+    front of every tensor, one per batch entry. Value head h reads key head
+    ``h // (heads // key_heads)``.
+
+    q, k, v: fp16 or bf16 of one type, any strides with contiguous heads
+    (others are copied); dk (up to 256) and dv multiples of 8. ``g`` (log
+    decay, -inf allowed) and ``beta`` in float32. ``initial_state`` (sequences,
+    heads, dk, dv) float32, zeros if None; the final state is a new tensor of
+    that shape. ``scale`` defaults to ``dk ** -0.5``. ``normalize_qk`` divides
+    each q and k by ``sqrt(sum of squares + 1e-6)`` first. No autograd: with
+    gradients enabled, inputs that require one are refused.
+    """
+    if not q.is_cuda:
+        require_cuda(q.device)
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    if q.dim() == 4:
+        if cu_seqlens is not None:
+            raise ValueError("cu_seqlens goes with packed tokens, not with a batch dimension")
+        if not (k.dim() == v.dim() == 4 and g.dim() == beta.dim() == 3):
+            raise ValueError("q, k, v must be (batch, tokens, heads, dim) and g, beta "
+                             "(batch, tokens, heads)")
+        batch, tokens = q.shape[:2]
+        for name, t in (("k", k), ("v", v), ("g", g), ("beta", beta)):
+            if t.shape[:2] != (batch, tokens):
+                raise ValueError(f"{name} must have q's batch and tokens, got {tuple(t.shape)}")
+        cu = torch.arange(0, (batch + 1) * tokens, max(tokens, 1), dtype=torch.int32,
+                          device=q.device) if tokens else \
+            torch.zeros(batch + 1, dtype=torch.int32, device=q.device)
+        o, state = ext().gated_delta_rule(q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1),
+                                          g.flatten(0, 1), beta.flatten(0, 1), cu, initial_state,
+                                          scale, normalize_qk)
+        return o.view(batch, tokens, *o.shape[1:]), state
+    if cu_seqlens is None:
+        cu_seqlens = torch.arange(0, q.shape[0] + 1, max(q.shape[0], 1), dtype=torch.int32,
+                                  device=q.device) if q.shape[0] else \
+            torch.zeros(2, dtype=torch.int32, device=q.device)
+    return ext().gated_delta_rule(q, k, v, g, beta, cu_seqlens, initial_state, scale, normalize_qk)
+
+
+def gated_delta_step_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor,
+                      beta: torch.Tensor, state: torch.Tensor,
+                      slots: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                      normalize_qk: bool = False) -> torch.Tensor:
+    """Outputs of one token of each of n sequences; ``state`` moves on in place.
+
+    ``q`` and ``k`` (n, key_heads, dk), ``v`` (n, heads, dv), ``g`` and
+    ``beta`` (n, heads) as in :func:`gated_delta_rule`; ``state`` (n, heads,
+    dk, dv) float32, contiguous. With ``slots`` (int32, n) ``state`` is a pool
+    and token i uses ``state[slots[i]]``; a slot outside the pool (a padded
+    entry, -1) leaves the pool alone and gets zeros. Two tokens of one call
+    must not share a slot.
+    """
+    if not q.is_cuda:
+        require_cuda(q.device)
+    return ext().gated_delta_step_(q, k, v, g, beta, state, slots,
+                                   q.shape[-1] ** -0.5 if scale is None else scale, normalize_qk)

@@ -1,0 +1,47 @@
+"""The norms around a decoder block on B200, fused with the block's gate and
+the scaled residual sum (``exl3_block_norm``): one pass over the rows where
+the calibration model takes a kernel per product.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from ._ext import ext, require_cuda
+
+_ACTIVATIONS = {"sigmoid": 1, "silu": 2}
+
+
+def block_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
+               gate: Optional[torch.Tensor] = None, gate_activation: str = "silu",
+               residual: Optional[torch.Tensor] = None, residual_scale: float = 1.0,
+               scale: Optional[torch.Tensor] = None,
+               next_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+               weight_offset: float = 0.0
+               ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """``(hidden, normed)`` of a block's output ``x`` (..., d)::
+
+        y = x / sqrt(mean(x^2) + eps) * (weight_offset + weight)   with weight, else x
+        y = y * act(gate)                                          with gate
+        hidden = residual + residual_scale * scale * y             with residual, else y
+        normed = hidden / sqrt(mean(hidden^2) + eps) * (weight_offset + next_weight)
+
+    Every part may be left out (a norm alone is ``next_weight``; then
+    ``hidden`` is ``x`` itself and ``normed`` None without ``next_weight``).
+    ``x``, ``gate`` and ``residual`` share shape and type (fp16, bf16, fp32);
+    ``weight``, ``next_weight`` and ``scale`` are vectors of d elements of
+    that type or float32 (one type for all); ``scale`` and ``residual_scale``
+    belong to the residual sum. Everything is computed in fp32 (the second
+    norm on hidden before its rounding) and each output rounded once. No
+    autograd: with gradients enabled, inputs that require one are refused.
+    """
+    if not x.is_cuda:
+        require_cuda(x.device)
+    act = _ACTIVATIONS.get(gate_activation)
+    if act is None:
+        raise ValueError(f"gate_activation must be one of {tuple(_ACTIVATIONS)}, "
+                         f"got {gate_activation!r}")
+    return ext().block_norm(x, weight, gate, act, residual, residual_scale, scale, next_weight,
+                            eps, weight_offset)

@@ -1,0 +1,123 @@
+"""Rotary positions on B200.
+
+``rotary_frequencies`` gives the angular frequencies of a head (plain, or
+scaled for contexts longer than the model was trained on); ``apply_rotary``
+turns queries and keys in one launch (``exl3_rotary``): both pair layouts,
+part of the head, any positions. The calibration model's
+``make_rotary_embeddings`` (``exl3_quant/calibration.py``) is the plain half
+layout with fp16 tables; here angles are exact at any position and every
+output is rounded once.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional, Sequence, Tuple
+
+import torch
+
+from ._ext import ext, require_cuda
+
+ROTARY_SCALINGS = ("none", "linear", "ntk", "yarn", "banded", "per_frequency")
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 500000.0, scaling: str = "none",
+                       factor: float = 1.0, original_length: int = 8192,
+                       beta_fast: float = 32.0, beta_slow: float = 1.0,
+                       low_freq_factor: float = 1.0, high_freq_factor: float = 4.0,
+                       frequency_factors: Optional[Sequence[float]] = None,
+                       device: Optional[torch.device] = None) -> Tuple[torch.Tensor, float]:
+    """``(inv_freq, attention_factor)`` for :func:`apply_rotary`: float32
+    radians per position of the ``rotary_dim / 2`` pairs, computed in float64,
+    and the factor on the rotated queries and keys.
+
+    ``scaling`` extends a model trained on ``original_length`` positions by
+    ``factor``:
+
+    * ``"none"``: ``base ** (-2 j / rotary_dim)``;
+    * ``"linear"``: every frequency divided by ``factor``;
+    * ``"ntk"``: the base grown by ``factor ** (d / (d - 2))``, so that the
+      lowest frequency is divided by ``factor`` and the highest kept;
+    * ``"yarn"``: frequencies that turn more than ``beta_fast`` times over
+      the original length kept, fewer than ``beta_slow`` times divided, a
+      linear ramp over the pair index between them; attention factor
+      ``0.1 ln(factor) + 1``;
+    * ``"banded"``: wavelengths shorter than ``original_length /
+      high_freq_factor`` kept, longer than ``original_length /
+      low_freq_factor`` divided, a ramp over the number of turns between;
+    * ``"per_frequency"``: each frequency divided by its own entry of
+      ``frequency_factors``; attention factor
+      ``sqrt(1 + ln(factor) / ln(original_length))`` for ``factor > 1``.
+    """
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be positive and even, got {rotary_dim}")
+    if scaling not in ROTARY_SCALINGS:
+        raise ValueError(f"scaling must be one of {ROTARY_SCALINGS}, got {scaling!r}")
+    if not (base > 1.0 and math.isfinite(base)):
+        raise ValueError(f"base must be finite and above 1, got {base}")
+    if not (factor >= 1.0 and math.isfinite(factor)):
+        raise ValueError(f"factor must be finite and at least 1, got {factor}")
+    if original_length < 1:
+        raise ValueError(f"original_length must be positive, got {original_length}")
+    half = rotary_dim // 2
+    j = torch.arange(half, dtype=torch.float64)
+    attention_factor = 1.0
+    if scaling == "ntk":
+        if rotary_dim < 4:
+            raise ValueError("ntk scaling needs a rotary_dim of at least 4")
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    inv = base ** (-j / half)
+    turns = original_length * inv / (2 * math.pi)  # over the original length
+    if scaling == "linear":
+        inv = inv / factor
+    elif scaling == "yarn":
+        if not beta_fast > beta_slow > 0:
+            raise ValueError("yarn scaling needs beta_fast > beta_slow > 0")
+
+        def index(count: float) -> float:  # the pair that turns `count` times
+            return half * math.log(original_length / (2 * math.pi * count)) / math.log(base)
+
+        lo = max(math.floor(index(beta_fast)), 0)
+        hi = min(math.ceil(index(beta_slow)), rotary_dim - 1)
+        ramp = ((j - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        inv = inv * (1 - ramp) + inv / factor * ramp
+        attention_factor = 0.1 * math.log(factor) + 1.0
+    elif scaling == "banded":
+        if not high_freq_factor > low_freq_factor > 0:
+            raise ValueError("banded scaling needs high_freq_factor > low_freq_factor > 0")
+        keep = ((turns - low_freq_factor) / (high_freq_factor - low_freq_factor)).clamp(0, 1)
+        inv = inv * keep + inv / factor * (1 - keep)
+    elif scaling == "per_frequency":
+        if frequency_factors is None or len(frequency_factors) != half:
+            raise ValueError(f"per_frequency scaling needs {half} frequency_factors")
+        inv = inv / torch.tensor(list(frequency_factors), dtype=torch.float64)
+        if factor > 1.0:
+            if original_length < 2:
+                raise ValueError("per_frequency scaling needs original_length of at least 2")
+            attention_factor = math.sqrt(1 + math.log(factor) / math.log(original_length))
+    return inv.to(device=device, dtype=torch.float32), attention_factor
+
+
+def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
+                 inv_freq: torch.Tensor, attention_factor: float = 1.0, interleaved: bool = False,
+                 heads_first: bool = False, transposed: bool = False, inplace: bool = False
+                 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Queries and keys turned by their positions, ``(q', k')``.
+
+    ``q`` and ``k`` are (batch, tokens, heads, dim), (batch, heads, tokens,
+    dim) with ``heads_first``, or (tokens, heads, dim) ((heads, tokens, dim));
+    fp16, bf16 or fp32, any strides with contiguous heads (others are
+    copied). ``k`` may be None. ``positions`` (int32 or int64) is (tokens) or
+    (batch, tokens). The first ``2 * len(inv_freq)`` elements of a head turn,
+    as pairs of its two halves or of neighbours (``interleaved``); the rest is
+    copied. ``transposed`` applies the transposed map: the gradient with
+    respect to q and k of a loss whose gradient is given. ``inplace`` writes
+    into q and k.
+
+    Angles are exact for any int64 position; products in fp32, one rounding.
+    No autograd: with gradients enabled, inputs that require one are refused.
+    """
+    if not q.is_cuda:
+        require_cuda(q.device)
+    return ext().apply_rotary(q, k, positions, inv_freq, attention_factor, interleaved,
+                              heads_first, transposed, inplace)

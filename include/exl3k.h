@@ -1,7 +1,8 @@
 /*
  * exl3k.h — C ABI of libexl3k, the B200 (sm_100a) kernels behind the EXL3
  * conversion hot path: the 16x16-tile trellis Viterbi encoder, the LDLQ
- * block-feedback helpers and the Hessian calibration accumulation.
+ * block-feedback helpers, the Hessian calibration accumulation and the layer
+ * operators between the linear projections of a calibration forward pass.
  *
  * Conventions (mirroring the reference op binding
  * csrc/quantize_xpu/quantize_xpu.cpp:73-101 of alpha2beta/EXL3_Intel_Arc_quantizer):
@@ -286,6 +287,100 @@ int exl3_regularize(const float* W, const float* su_in, const float* sv_in,
  */
 int exl3_block_ldl_fold(const float* chol, float* L, float* inverses, int64_t n,
                         exl3_stream_t stream);
+
+/* ------------------------------------------------------------------ */
+/* Decoder-layer operators between the linear projections              */
+/* ------------------------------------------------------------------ */
+
+/* Element types of the operators below. */
+enum { EXL3_F16 = 0, EXL3_BF16 = 1, EXL3_F32 = 2 };
+
+/*
+ * Rotary positions on queries and keys in one launch. With phi = position *
+ * inv_freq[j], j < rotary_dim / 2, and the pair (a, b) = (x[j],
+ * x[j + rotary_dim / 2]) or, interleaved, (x[2j], x[2j + 1]):
+ *   a' = factor (a cos phi - b sin phi),  b' = factor (b cos phi + a sin phi);
+ * elements from rotary_dim on are copied. `transposed` negates the sine: the
+ * transposed map, which is the gradient's. The angle is reduced exactly (a
+ * 64-bit fixed-point fraction of a turn), so it does not lose precision at
+ * large positions. Products in fp32, one rounding at the end.
+ */
+typedef struct exl3_rotary_args {
+  const void *q, *k;       /* dim contiguous elements per head; k may be NULL with k_heads = 0 */
+  void *q_out, *k_out;     /* may be q and k themselves with the same strides */
+  const void* positions;   /* int32, or int64 with positions_64 */
+  const float* inv_freq;   /* rotary_dim / 2 radians per position */
+  int64_t batch, tokens;
+  int64_t q_strides[3], k_strides[3], q_out_strides[3], k_out_strides[3]; /* batch, token, head */
+  int64_t position_strides[2];                                           /* batch (0: shared), token */
+  int q_heads, k_heads, dim, rotary_dim;
+  int dtype;               /* EXL3_F16, EXL3_BF16 or EXL3_F32 */
+  int positions_64, interleaved, transposed;
+  float factor;
+} exl3_rotary_args;
+int exl3_rotary(const exl3_rotary_args* args, exl3_stream_t stream);
+
+/*
+ * The norm after a block, its gate, the scaled residual sum and the norm
+ * before the next block, row by row, in one pass:
+ *   y = weight ? x / sqrt(mean(x^2) + eps) * (weight_offset + weight) : x
+ *   y = gate ? y * act(gate) : y
+ *   h = residual ? residual + residual_scale * (scale ? scale : 1) * y : y
+ *   hidden = h,  normed = h / sqrt(mean(h^2) + eps) * (weight_offset + next_weight)
+ * everything in fp32, each output rounded once. hidden may be NULL (not
+ * stored); normed is written where next_weight is given.
+ */
+typedef struct exl3_block_norm_args {
+  const void *x, *gate, *residual;          /* (rows, d) of dtype; gate and residual may be NULL */
+  const void *weight, *next_weight, *scale; /* (d) of param_dtype; may be NULL */
+  void *hidden, *normed;                    /* (rows, d) of dtype */
+  int64_t rows, d;
+  int64_t x_stride, gate_stride, residual_stride, hidden_stride, normed_stride; /* elements */
+  int dtype, param_dtype;                   /* param_dtype: dtype or EXL3_F32 */
+  int gate_activation;                      /* 0 none, 1 sigmoid, 2 silu */
+  float eps, weight_offset, residual_scale;
+} exl3_block_norm_args;
+int exl3_block_norm(const exl3_block_norm_args* args, exl3_stream_t stream);
+
+/*
+ * The gated delta rule. For each value head h (reading key head
+ * h / (heads / key_heads)), with the state S (dk, dv) held in fp32:
+ *   S_t = e^{g_t} S_{t-1} + k_t u_t^T,  u_t = beta_t (v_t - e^{g_t} S_{t-1}^T k_t)
+ *   o_t = scale S_t^T q_t
+ * normalize_qk divides each q and k by sqrt(sum of squares + 1e-6) first.
+ * dk and dv are multiples of 8, dk <= 256.
+ *
+ * exl3_delta_step: one token of each of `seqs` sequences, in place on the
+ * states. slots (int32, may be NULL: slot = sequence) picks each sequence's
+ * state among num_slots; a slot outside [0, num_slots) leaves the states
+ * alone and writes zeros. Two sequences of one call do not share a slot.
+ *
+ * exl3_delta_rule: whole sequences, packed: sequence s is the tokens
+ * cu_seqlens[s] .. cu_seqlens[s + 1] (device, not read by the host; bounds
+ * outside [0, tokens] are clamped). state_in (may be NULL: zeros) and
+ * state_out are (seqs, heads, dk, dv). exl3_delta_rule_ws_bytes returns the
+ * workspace size (0 on invalid arguments; a valid call may need none and then
+ * reports 16).
+ */
+typedef struct exl3_delta_args {
+  const void *q, *k;        /* (tokens, key_heads, dk) of dtype */
+  const void* v;            /* (tokens, heads, dv) of dtype */
+  const float *g, *beta;    /* (tokens, heads) */
+  const float* state_in;
+  float* state_out;
+  void* out;                /* (tokens, heads, dv) of dtype, contiguous */
+  const int32_t *cu_seqlens, *slots;
+  int64_t tokens, seqs, num_slots;
+  int64_t q_strides[2], k_strides[2], v_strides[2]; /* token, head */
+  int64_t g_stride, beta_stride;                    /* token */
+  int key_heads, heads, dk, dv;
+  int dtype;                /* EXL3_F16 or EXL3_BF16 */
+  int normalize_qk;
+  float scale;
+} exl3_delta_args;
+int exl3_delta_step(const exl3_delta_args* args, exl3_stream_t stream);
+size_t exl3_delta_rule_ws_bytes(const exl3_delta_args* args);
+int exl3_delta_rule(const exl3_delta_args* args, void* ws, size_t ws_bytes, exl3_stream_t stream);
 
 /* ------------------------------------------------------------------ */
 /* Diagnostics                                                         */
