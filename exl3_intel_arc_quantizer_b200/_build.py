@@ -34,7 +34,7 @@ LIB_NAME = "libexl3k.so"
 EXT_NAME = "exl3_b200_ext"
 
 CU_SOURCES = ["abi.cu", "encoder.cu", "acs_pair.cu", "acs_cluster.cu", "noalloc.cu", "linalg.cu", "hessian.cu", "storage.cu", "ldlq.cu", "regularize.cu",
-              "rotary.cu", "block_norm.cu", "delta_rule.cu"]
+              "rotary.cu", "block_norm.cu", "delta_rule.cu", "delta_chunk.cu"]
 EXT_SOURCES = ["torch_ext.cpp", "torch_ext_linalg.cpp", "torch_ext_layer.cpp"]
 
 NVCC_FLAGS = [

@@ -166,6 +166,9 @@ int launch_tokens(const exl3_delta_args& a, cudaStream_t stream) {
   return EXL3_OK;
 }
 
+// The chunked form for all but a handful of tokens and heads too wide for it.
+bool chunked(const exl3_delta_args& a) { return a.dk <= 128 && a.tokens > 8; }
+
 int check_args(const exl3_delta_args* args) {
   EXL3_REQUIRE(args != nullptr, "args is NULL");
   const exl3_delta_args& a = *args;
@@ -210,7 +213,7 @@ extern "C" int exl3_delta_step(const exl3_delta_args* args, exl3_stream_t stream
 
 extern "C" size_t exl3_delta_rule_ws_bytes(const exl3_delta_args* args) {
   if (check_args(args)) return 0;
-  return 16;
+  return chunked(*args) ? delta_chunk_ws_bytes(*args) : 16;
 }
 
 extern "C" int exl3_delta_rule(const exl3_delta_args* args, void* ws, size_t ws_bytes,
@@ -224,6 +227,10 @@ extern "C" int exl3_delta_rule(const exl3_delta_args* args, void* ws, size_t ws_
   EXL3_REQUIRE(a.cu_seqlens, "cu_seqlens is NULL");
   if (const int rc = check_pointers(a)) return rc;
   cudaStream_t s = (cudaStream_t)stream;
+  if (chunked(a)) {
+    EXL3_REQUIRE(aligned_to(ws, 16), "the workspace must be 16-byte aligned");
+    return delta_chunks(a, ws, s);
+  }
   return a.dtype == EXL3_F16 ? launch_tokens<__half, false>(a, s)
                              : launch_tokens<__nv_bfloat16, false>(a, s);
 }

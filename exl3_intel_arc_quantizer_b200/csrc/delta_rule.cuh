@@ -8,6 +8,10 @@ namespace exl3 {
 
 constexpr float kNormEps = 1e-6f;  // added to a sum of squares of q or k
 
+// The chunked form (delta_chunk.cu); dk <= 128.
+size_t delta_chunk_ws_bytes(const exl3_delta_args& a);
+int delta_chunks(const exl3_delta_args& a, void* ws, cudaStream_t stream);
+
 // Tokens [t0, t1) of sequence s. The offsets are device data that the host
 // has not seen: they are clamped into [0, tokens], and a sequence that would
 // end before it begins is empty.
