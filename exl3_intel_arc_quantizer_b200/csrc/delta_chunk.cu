@@ -54,17 +54,21 @@ namespace {
 
 constexpr int kChunk = 64;
 constexpr int kImageBytes = 128 * 128 * 2;  // [T; P T]: 128 rows x 64, high and low parts
-// per chunk and head: a (64), b (64), c (64), the scalars, and the factors of
-// the 64 k and 64 q rows on their way to fp16
-constexpr int kVecFloats = 384;
+constexpr int kKqBytes = 128 * 128 * 2;     // [K; Q] in fp16: two tiles of 128 rows x 64 of dk
+// per chunk and head: a (64), b (64), c (64) and the scalars
+constexpr int kVecFloats = 256;
 constexpr int kGamma = 192, kBoundA = 193, kBoundU = 194, kBoundS = 195, kScaleT = 196,
-              kScalePT = 197, kRowScale = 256;
-constexpr int64_t kSlotBytes = kImageBytes + kVecFloats * 4;
+              kScalePT = 197;
+constexpr int64_t kHeadBytes = kImageBytes + kVecFloats * 4;
 
 // Chunk c of a sequence that begins at token t0 has workspace slot
 // t0 / 64 + s + c: sequences never share one, and there are tokens / 64 +
-// seqs of them, whatever the lengths.
+// seqs of them, whatever the lengths. A slot holds its key heads' [K; Q], then
+// its heads' images and vectors.
 __device__ __forceinline__ int64_t slot_base(int64_t t0, int64_t s) { return t0 / kChunk + s; }
+__host__ __device__ __forceinline__ int64_t slot_bytes(const exl3_delta_args& a) {
+  return (int64_t)a.key_heads * kKqBytes + (int64_t)a.heads * kHeadBytes;
+}
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -77,18 +81,17 @@ __device__ __forceinline__ uint32_t swz(int r, int q) {
 }
 
 // x = hi + lo, two fp16 parts each
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
-  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+__device__ __forceinline__ void split2(float2 x, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __float22half2_rn(x);
+  const __half2 l = __float22half2_rn(__ffma2_rn(__half22float2(h), make_float2(-1.f, -1.f), x));
   hi = *reinterpret_cast<const uint32_t*>(&h);
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
-__device__ __forceinline__ void split8(const float* x, uint4& hi, uint4& lo) {
-  split2(x[0], x[1], hi.x, lo.x);
-  split2(x[2], x[3], hi.y, lo.y);
-  split2(x[4], x[5], hi.z, lo.z);
-  split2(x[6], x[7], hi.w, lo.w);
+__device__ __forceinline__ void split8(const float2* x, uint4& hi, uint4& lo) {
+  split2(x[0], hi.x, lo.x);
+  split2(x[1], hi.y, lo.y);
+  split2(x[2], hi.z, lo.z);
+  split2(x[3], hi.w, lo.w);
 }
 
 // The power of two that puts a bound (>= 0) into [2^14, 2^15), and its
@@ -256,6 +259,29 @@ delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict
     }
   }
   __syncthreads();
+  // [K; Q] as the chain's operand, zeros up to the tiles' ends
+  {
+    uint8_t* dst = ws + slot * slot_bytes(a) + (int64_t)kh * kKqBytes;
+    for (int i = tid; i < 128 * 16; i += kPrepThreads) {
+      const int r = i >> 4, q = i & 15;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (q < pieces) {
+        x = *reinterpret_cast<const uint4*>(&sm.u.kq[r >> 6][r & 63][8 * q]);
+        if constexpr (!std::is_same<T, __half>::value) {
+          const float f = sm.rowscale[r];
+          const T* e = reinterpret_cast<const T*>(&x);
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const __half2 p = __floats2half2_rn(to_f32(e[2 * j]) * f, to_f32(e[2 * j + 1]) * f);
+            w[j] = *reinterpret_cast<const uint32_t*>(&p);
+          }
+          x = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      *reinterpret_cast<uint4*>(dst + (q >> 3) * (kKqBytes / 2) + swz(r, q & 7)) = x;
+    }
+  }
   if (tid < kChunk) sm.rk[tid] = a.normalize_qk ? rsqrtf(sm.dot[0][tid][tid] + kNormEps) : 1.f;
   float knorm[2] = {0.f, 0.f};  // |k| of rows 2 lane and 2 lane + 1
   if (warp == 0) {
@@ -371,7 +397,7 @@ delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict
     }
     __syncthreads();
     // T = X beta into M's place, P T into tmp-free registers: a 4x4 tile each
-    uint8_t* img = ws + (slot * a.heads + h) * kSlotBytes;
+    uint8_t* img = ws + slot * slot_bytes(a) + (int64_t)a.key_heads * kKqBytes + h * kHeadBytes;
     {
       const int r = 4 * (tid >> 4), c = 4 * (tid & 15);
       float v[4][4];
@@ -445,20 +471,19 @@ delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint2 hi, lo;
-        split2(x[i][0] * st, x[i][1] * st, hi.x, lo.x);
-        split2(x[i][2] * st, x[i][3] * st, hi.y, lo.y);
+        split2(make_float2(x[i][0] * st, x[i][1] * st), hi.x, lo.x);
+        split2(make_float2(x[i][2] * st, x[i][3] * st), hi.y, lo.y);
         const uint32_t at = swz(r + i, c >> 3) + 2 * (c & 7);
         *reinterpret_cast<uint2*>(img + at) = hi;
         *reinterpret_cast<uint2*>(img + kImageBytes / 2 + at) = lo;
-        split2(v[i][0] * sp, v[i][1] * sp, hi.x, lo.x);
-        split2(v[i][2] * sp, v[i][3] * sp, hi.y, lo.y);
+        split2(make_float2(v[i][0] * sp, v[i][1] * sp), hi.x, lo.x);
+        split2(make_float2(v[i][2] * sp, v[i][3] * sp), hi.y, lo.y);
         const uint32_t at2 = swz(64 + r + i, c >> 3) + 2 * (c & 7);
         *reinterpret_cast<uint2*>(img + at2) = hi;
         *reinterpret_cast<uint2*>(img + kImageBytes / 2 + at2) = lo;
       }
     }
     float* vout = reinterpret_cast<float*>(img + kImageBytes);
-    if (tid >= 64 && tid < 192) vout[kRowScale + tid - 64] = sm.rowscale[tid - 64];
     if (warp == 0) {
       float ba = 0.f, bu = 0.f, bs = 0.f;
 #pragma unroll
@@ -499,41 +524,39 @@ delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict
 // The chain of states
 // ---------------------------------------------------------------------------
 
-constexpr uint64_t kWaitNs = 2000000000ull;  // 2 s per wait
+constexpr long long kWaitClocks = 4000000000ll;  // 2 s per wait at 2 GHz
 
 // GROUPS column groups of NV columns, each with its own barriers, tensor
-// memory and issuing thread (one group's products run under the other's
-// elementwise steps); CT columns per epilogue thread. NV = 32 keeps the high
-// and low parts of an operand side by side as 64 columns (their products
-// land in separate columns and are added in the epilogue); NV = 64 keeps two
-// operands, whose products accumulate.
-template <typename T, int GROUPS, int NV, int CT>
+// memory and issuing warp (one group's products run under the other's
+// elementwise steps); CT columns per epilogue thread. The high and low parts
+// of an operand stand side by side as 2 NV columns (two tiles, or for NV = 32
+// the halves of one): the 4 KB of the other operand that a K = 16 product
+// reads from shared memory (32 clocks) then serve both, and the two results,
+// in separate columns, are added in the epilogue.
+template <int GROUPS, int NV, int CT>
 struct Geo {
-  static constexpr bool kPacked = NV == 32;
   static constexpr int kWG = NV / CT;                    // epilogue warpgroups of a group
   static constexpr int kEpiWarps = 4 * kWG * GROUPS;
-  static constexpr int kProducers = GROUPS == 2 ? 2 : 4;  // warps
-  static constexpr int kThreads = 32 * (kEpiWarps + GROUPS + kProducers);
-  static constexpr int kBox = 128 * 128;                 // [K; Q]: 128 rows x 64 of dk
-  static constexpr int kKQ = 2 * kBox;
+  static constexpr int kThreads = 32 * (kEpiWarps + GROUPS + 1);
+  static constexpr int kBox = kKqBytes / 2;              // [K; Q]: 128 rows x 64 of dk
   static constexpr int kKQStages = 2;
-  static constexpr int kTStages = 2;
-  static constexpr int kPartsB = kPacked ? 1 : 2;        // operand tiles of S, R, U
-  static constexpr int kSBytes = 128 * 128 * kPartsB;
-  static constexpr int kRBytes = 64 * 128 * kPartsB;
-  static constexpr int kCols = 3 * 64;                   // tensor memory of a group
-  static constexpr int kAlloc = GROUPS == 2 ? 512 : 256;
-  static constexpr int kBars = 2 * kKQStages + 2 * kTStages + 7 * GROUPS;
-  static constexpr size_t kSmem = 1024 + (size_t)kKQStages * kKQ + kTStages * kImageBytes +
-                                  GROUPS * (kSBytes + kRBytes) + kBars * 8 + 16 + 32;
+  static constexpr int kTStages = 2;                     // images with their vectors, and v
+  static constexpr int kVRow = GROUPS * NV * 2;          // bytes of a row of v, pieces swizzled
+  static constexpr int kVBytes = kChunk * kVRow;
+  static constexpr int kTBytes = kHeadBytes + kVBytes;
+  // S, then R and c U: each is written after the products that read the one
+  // before it have finished
+  static constexpr int kOpBytes = NV == 32 ? 128 * 128 : 2 * 128 * 128;
+  static constexpr int kCols = 4 * NV;                   // tensor memory of a group
+  static constexpr int kAlloc = GROUPS * kCols;
+  static_assert(kAlloc == 128 || kAlloc == 512, "power of two");
+  static constexpr int kBars = 2 * kKQStages + 2 * kTStages + 8 * GROUPS;
+  static constexpr size_t kSmem = (size_t)kKQStages * kKqBytes + kTStages * kTBytes +
+                                  GROUPS * kOpBytes + kBars * 8 + 16 + 32;
+  static_assert(kTBytes % 1024 == 0 && kOpBytes % 1024 == 0, "operand tiles start on 1,024 bytes");
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
-__device__ __forceinline__ uint64_t gtimer() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
 }
@@ -554,13 +577,14 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
 // true when the phase completed; false on timeout (which raises the abort
 // flag) or when another role has aborted
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  if (bar_try(bar, parity)) return true;
-  const uint64_t start = gtimer();
-  for (uint32_t it = 0;; ++it) {
+  long long start = 0;
+  for (uint32_t it = 1;; ++it) {
     if (bar_try(bar, parity)) return true;
-    if ((it & 31u) == 31u) {
+    if ((it & 63u) == 0u) {
       if (*abort_flag) return false;
-      if (gtimer() - start > kWaitNs) {
+      const long long now = clock64();
+      if (start == 0) start = now;
+      if (now - start > kWaitClocks) {
         *abort_flag = 1;
         return false;
       }
@@ -569,44 +593,53 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
 }
 // the shutdown path's wait: bounded, whatever the abort flag says
 __device__ __forceinline__ void bar_drain(uint32_t bar, uint32_t parity) {
-  const uint64_t start = gtimer();
+  const long long start = clock64();
   while (!bar_try(bar, parity))
-    if (gtimer() - start > kWaitNs) return;
+    if (clock64() - start > kWaitClocks) return;
 }
 
-// 128-byte-swizzled operand: 8-row groups 1,024 bytes apart; lbo is the
-// distance of the next 64 rows or columns of an operand whose M or N runs
-// along the 128 bytes (not used along K)
-__device__ __forceinline__ uint64_t desc(uint32_t saddr, uint32_t lbo) {
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)((lbo >> 4) & 0x3FFF) << 16) |
-         ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// Operand descriptor of a 128-byte-swizzled tile (8-row groups 1,024 bytes
+// apart): this is the low word, the high one is kDescHigh. lbo is the distance
+// of the next 64 rows or columns of an operand whose M or N runs along the 128
+// bytes (not used along K).
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc(uint32_t saddr, uint32_t lbo) {
+  return ((saddr >> 4) & 0x3FFF) | ((lbo >> 4) << 16);
 }
 // fp16 x fp16 -> fp32, M = 128; B's N along the 128 bytes, A's K or M
 __host__ __device__ constexpr uint32_t idesc(int n, bool a_m_major) {
-  return (1u << 4) | ((a_m_major ? 1u : 0u) << 15) | (1u << 16) |
-         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+  return (1u << 4) | ((a_m_major ? 1u : 0u) << 15) | (1u << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(128 >> 4) << 24);
 }
-__device__ __forceinline__ void mma(uint32_t d, uint64_t da, uint64_t db, uint32_t id, bool add) {
+// Called by the whole warp, issued by its elected lane: every operand stays
+// in uniform registers (behind a branch on the lane each product took about
+// 95 clocks to issue).
+template <bool ADD>
+__device__ __forceinline__ void mma(uint32_t d, uint32_t da, uint32_t db, uint32_t id, uint32_t elected) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(da), "l"(db), "r"(id), "r"((uint32_t)add));
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "mov.b64 a, {%1, %6};\n\tmov.b64 b, {%2, %6};\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, q;\n\t}" ::"r"(d),
+      "r"(da), "r"(db), "r"(id), "r"(elected), "n"(ADD ? 1 : 0), "n"(kDescHigh));
 }
-__device__ __forceinline__ void commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-               : "memory");
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e;
 }
-__device__ __forceinline__ void tmem_ld(uint32_t addr, float (&f)[16]) {
-  uint32_t v[16];
+__device__ __forceinline__ void commit(uint32_t bar, uint32_t elected) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
-        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
-        "=r"(v[14]), "=r"(v[15])
-      : "r"(addr));
-#pragma unroll
-  for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+      "@p tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+      "r"(elected)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld(uint32_t addr, float2 (&f)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=f"(f[0].x), "=f"(f[0].y), "=f"(f[1].x), "=f"(f[1].y), "=f"(f[2].x), "=f"(f[2].y),
+                 "=f"(f[3].x), "=f"(f[3].y)
+               : "r"(addr));
 }
 __device__ __forceinline__ void tmem_ld_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -622,12 +655,11 @@ __device__ __forceinline__ void fence_after() {
 }
 
 template <typename T, int GROUPS, int NV, int CT>
-__global__ void __launch_bounds__(Geo<T, GROUPS, NV, CT>::kThreads, 1)
+__global__ void __launch_bounds__(Geo<GROUPS, NV, CT>::kThreads, 1)
 delta_chain_kernel(const __grid_constant__ exl3_delta_args a, const uint8_t* __restrict__ ws,
                    int vec) {
-  using L = Geo<T, GROUPS, NV, CT>;
-  constexpr bool kPacked = L::kPacked;
-  extern __shared__ uint8_t dsm[];
+  using L = Geo<GROUPS, NV, CT>;
+  extern __shared__ __align__(1024) uint8_t chain_smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int slices = (a.dv + GROUPS * NV - 1) / (GROUPS * NV);
   const int slice = blockIdx.x % slices;
@@ -662,16 +694,19 @@ delta_chain_kernel(const __grid_constant__ exl3_delta_args a, const uint8_t* __r
     return;
   }
   const int chunks = (int)((t1 - t0 + kChunk - 1) / kChunk);
-  const uint8_t* img = ws + (slot_base(t0, s) * a.heads + h) * kSlotBytes;
-  const int64_t img_step = (int64_t)a.heads * kSlotBytes;
+  const int64_t img_step = slot_bytes(a);
+  const uint8_t* kq_img = ws + slot_base(t0, s) * img_step + (int64_t)kh * kKqBytes;
+  const uint8_t* img =
+      ws + slot_base(t0, s) * img_step + (int64_t)a.key_heads * kKqBytes + h * kHeadBytes;
 
-  uint8_t* smem = reinterpret_cast<uint8_t*>(
-      (reinterpret_cast<uintptr_t>(dsm) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* kq_base = smem;
-  uint8_t* t_base = kq_base + L::kKQStages * L::kKQ;
-  uint8_t* s_base = t_base + L::kTStages * kImageBytes;
-  uint8_t* r_base = s_base + GROUPS * L::kSBytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(r_base + GROUPS * L::kRBytes);
+  if (smem_u32(chain_smem) & 1023) {  // the operand tiles' layout rests on it
+    if (tid == 0) atomicAdd(&g_delta_faults, 1u);
+    return;
+  }
+  uint8_t* kq_base = chain_smem;
+  uint8_t* t_base = kq_base + L::kKQStages * kKqBytes;
+  uint8_t* op_base = t_base + L::kTStages * L::kTBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(op_base + GROUPS * L::kOpBytes);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   // per group: bits of max |S| before step ch and of max |v| of it, by ch & 1
@@ -682,32 +717,30 @@ delta_chain_kernel(const __grid_constant__ exl3_delta_args a, const uint8_t* __r
   const auto t_full = [&](int st) { return bar(2 * L::kKQStages + st); };
   const auto t_empty = [&](int st) { return bar(2 * L::kKQStages + L::kTStages + st); };
   constexpr int kG0 = 2 * L::kKQStages + 2 * L::kTStages;
-  // per group: s, r, u ready (epilogue -> issuer), d1, d2, d3 (products), done
-  const auto gbar = [&](int g, int i) { return bar(kG0 + 7 * g + i); };
+  // per group: s, r, u ready (epilogue -> issuer), d1, d2, d3 (products), done,
+  // peaks noted (epilogue -> epilogue)
+  const auto gbar = [&](int g, int i) { return bar(kG0 + 8 * g + i); };
 
   if (tid == 0) {
     for (int i = 0; i < L::kKQStages; ++i) {
-      bar_init(kq_full(i), 32 * L::kProducers);
+      bar_init(kq_full(i), 1);
       bar_init(kq_empty(i), GROUPS);
     }
     for (int i = 0; i < L::kTStages; ++i) {
-      bar_init(t_full(i), 1);
-      bar_init(t_empty(i), GROUPS);
+      bar_init(t_full(i), 1 + 32);
+      bar_init(t_empty(i), GROUPS + L::kEpiWarps);
     }
     for (int g = 0; g < GROUPS; ++g) {
       bar_init(gbar(g, 0), 4 * L::kWG);
       bar_init(gbar(g, 1), 2 * L::kWG);
-      bar_init(gbar(g, 2), 2 * L::kWG);
+      bar_init(gbar(g, 2), 4 * L::kWG);
       for (int i = 3; i < 7; ++i) bar_init(gbar(g, i), 1);
+      bar_init(gbar(g, 7), 4 * L::kWG);
     }
     *abort_flag = 0;
     for (int i = 0; i < 4 * GROUPS; ++i) (&peak[0][0][0])[i] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  // columns past dk are read by the products and never written again
-  for (int i = tid; i < L::kKQStages * L::kKQ / 16; i += L::kThreads)
-    reinterpret_cast<uint4*>(kq_base)[i] = make_uint4(0, 0, 0, 0);
-  fence_async();
   if (warp == L::kEpiWarps) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(tmem_slot)),
@@ -726,33 +759,29 @@ delta_chain_kernel(const __grid_constant__ exl3_delta_args a, const uint8_t* __r
     const int col = col_base + g * NV + c0;           // in the state
     const int row = 32 * quarter + lane;              // of dk; of [K; Q]
     const bool lower = quarter < 2;                   // K S, U rows; the others Q S, O rows
-    uint8_t* s_op = s_base + g * L::kSBytes;
-    uint8_t* r_op = r_base + g * L::kRBytes;
+    uint8_t* op = op_base + g * L::kOpBytes;
     const uint32_t d1 = tmem + (uint32_t)(g * L::kCols) + ((uint32_t)(32 * quarter) << 16) + c0;
-    const uint32_t d2 = d1 + 64, d3 = d1 + 128;
-    // a product's columns c .. c + 15 of this thread's row
-    const auto product = [&](uint32_t d, int c, float (&f)[16]) {
+    const uint32_t d2 = d1 + 2 * NV, d3 = d2;  // U and P U are read before K^T U overwrites them
+    // a product's columns c .. c + 7 of this thread's row, both parts
+    const auto load2 = [&](uint32_t d, int c, float2 (&f)[4], float2 (&l)[4]) {
       tmem_ld(d + c, f);
-      if constexpr (kPacked) {
-        float l[16];
-        tmem_ld(d + 32 + c, l);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) f[i] += l[i];
-      } else {
-        tmem_ld_wait();
-      }
+      tmem_ld(d + NV + c, l);
     };
-    // 16 values into columns c .. c + 15 of row r of an operand, both parts
-    const auto store_op = [&](uint8_t* op, int tile, int r, int c, const float (&f)[16]) {
+    const auto add2 = [&](float2 (&f)[4], const float2 (&l)[4]) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        uint4 hi, lo;
-        split8(f + 8 * e, hi, lo);
-        const int q = (c0 + c) / 8 + e;
-        *reinterpret_cast<uint4*>(op + swz(r, q)) = hi;
-        *reinterpret_cast<uint4*>(kPacked ? op + swz(r, q + 4) : op + tile + swz(r, q)) = lo;
-      }
+      for (int i = 0; i < 4; ++i) f[i] = __fadd2_rn(f[i], l[i]);
+    };
+    // into columns c .. c + 7 of this row of an operand, both parts; tile:
+    // bytes between the parts' tiles
+    const auto store_op = [&](int tile, int c, const float2 (&f)[4], __half2& peak2) {
+      uint4 hi, lo;
+      split8(f, hi, lo);
+      const __half2* hp = reinterpret_cast<const __half2*>(&hi);
+      peak2 = __hmax2(peak2, __hmax2(__hmax2(__habs2(hp[0]), __habs2(hp[1])),
+                                     __hmax2(__habs2(hp[2]), __habs2(hp[3]))));
+      const int q = (c0 + c) / 8;
+      *reinterpret_cast<uint4*>(op + swz(row, q)) = hi;
+      *reinterpret_cast<uint4*>(NV == 32 ? op + swz(row, q + 4) : op + tile + swz(row, q)) = lo;
     };
     const auto ready = [&](int i) {
       fence_async();
@@ -760,46 +789,45 @@ delta_chain_kernel(const __grid_constant__ exl3_delta_args a, const uint8_t* __r
       __syncwarp();
       if (lane == 0) bar_arrive(gbar(g, i));
     };
-    float S[CT];
-    uint4 vr[CT / 8];
-    const T* v = static_cast<const T*>(a.v) + h * a.v_strides[1] + col;
+    float2 S[CT / 2];
     T* out = static_cast<T*>(a.out) + (int64_t)h * a.dv + col;
-    const auto load_v = [&](int ch) {
-      const int64_t t = t0 + (int64_t)ch * kChunk + row;
-#pragma unroll
-      for (int c = 0; c < CT / 8; ++c)
-        vr[c] = lower && t < t1 && col + 8 * c < a.dv ? load8(v + t * a.v_strides[0] + 8 * c, vec & 2)
-                                                      : make_uint4(0, 0, 0, 0);
+    // columns 8 c .. of this thread's v in step ch (piece q of row r stands at
+    // q ^ (r & 7), so that 8 rows of a piece use all banks)
+    const auto load_v = [&](int ch, int c) {
+      const uint8_t* tile = t_base + (ch % L::kTStages) * L::kTBytes + kHeadBytes;
+      const int q = (g * NV + c0) / 8 + c;
+      return *reinterpret_cast<const uint4*>(tile + row * L::kVRow + ((q ^ (row & L::kVRow / 16 - 1 & 7)) << 4));
     };
-    // the peaks that step ch starts from
-    const auto note_peaks = [&](int ch) {
-      float m = 0.f;
-#pragma unroll
-      for (int c = 0; c < CT; ++c) m = fmaxf(m, fabsf(S[c]));
-      const uint32_t ms = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(m));
-      if (lane == 0) atomicMax(&peak[g][ch & 1][0], ms);
+    const auto note_peak_v = [&](int ch) {
       if (lower) {
         uint32_t w = 0;  // 16-bit patterns of non-negative values order like the values
 #pragma unroll
         for (int c = 0; c < CT / 8; ++c) {
-          w = __vmaxu2(w, vr[c].x & 0x7FFF7FFFu);
-          w = __vmaxu2(w, vr[c].y & 0x7FFF7FFFu);
-          w = __vmaxu2(w, vr[c].z & 0x7FFF7FFFu);
-          w = __vmaxu2(w, vr[c].w & 0x7FFF7FFFu);
+          const uint4 x = load_v(ch, c);
+          w = __vmaxu2(w, x.x & 0x7FFF7FFFu);
+          w = __vmaxu2(w, x.y & 0x7FFF7FFFu);
+          w = __vmaxu2(w, x.z & 0x7FFF7FFFu);
+          w = __vmaxu2(w, x.w & 0x7FFF7FFFu);
         }
         const uint16_t top = (uint16_t)__reduce_max_sync(0xFFFFFFFFu, max(w & 0xFFFFu, w >> 16));
         if (lane == 0)
           atomicMax(&peak[g][ch & 1][1], __float_as_uint(to_f32(*reinterpret_cast<const T*>(&top))));
       }
     };
-    // S times its scale, as 16-column pieces (CT is 16 or 32)
+    const auto note_peak_s = [&](int ch, float m) {
+      const uint32_t ms = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(m));
+      if (lane == 0) atomicMax(&peak[g][ch & 1][0], ms);
+    };
+    // S times its scale; the largest |S| is taken from the high parts, which are within 2^-11 of it
+    __half2 peak2;
     const auto store_state = [&](float scale) {
+      peak2 = __half2half2(__ushort_as_half(0));
 #pragma unroll
-      for (int c = 0; c < CT; c += 16) {
-        float f[16];
+      for (int c = 0; c < CT; c += 8) {
+        float2 f[4];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) f[i] = S[c + i] * scale;
-        store_op(s_op, 128 * 128, row, c, f);
+        for (int i = 0; i < 4; ++i) f[i] = __fmul2_rn(S[c / 2 + i], make_float2(scale, scale));
+        store_op(128 * 128, c, f, peak2);
       }
     };
 #pragma unroll
@@ -807,53 +835,68 @@ delta_chain_kernel(const __grid_constant__ exl3_delta_args a, const uint8_t* __r
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
       if (a.state_in && row < a.dk && col + c < a.dv)
         x = *reinterpret_cast<const float4*>(a.state_in + state_at + (int64_t)row * a.dv + col + c);
-      S[c] = x.x;
-      S[c + 1] = x.y;
-      S[c + 2] = x.z;
-      S[c + 3] = x.w;
+      S[c / 2] = make_float2(x.x, x.y);
+      S[c / 2 + 1] = make_float2(x.z, x.w);
     }
-    load_v(0);
-    note_peaks(0);
-    asm volatile("bar.sync %0, %1;" ::"r"(1 + g), "n"(128 * L::kWG) : "memory");
+    bool ok = __all_sync(0xFFFFFFFFu, bar_wait(t_full(0), 0, abort_flag));
+    if (ok) {
+      float m = 0.f;
+#pragma unroll
+      for (int c = 0; c < CT / 2; ++c) m = fmaxf(m, fmaxf(fabsf(S[c].x), fabsf(S[c].y)));
+      note_peak_s(0, m);
+      note_peak_v(0);
+      __syncwarp();
+      if (lane == 0) bar_arrive(gbar(g, 7));
+      ok = __all_sync(0xFFFFFFFFu, bar_wait(gbar(g, 7), 0, abort_flag));
+    }
     float scale_s, inv_s;
     pow2_scale(__uint_as_float(peak[g][0][0]), scale_s, inv_s);
     store_state(scale_s);
     ready(0);
-    bool ok = true;
     for (int ch = 0; ch < chunks && ok; ++ch) {
       const uint32_t ph = ch & 1;
-      const float* vecs = reinterpret_cast<const float*>(img + ch * img_step + kImageBytes);
+      const int ts = ch % L::kTStages;
+      const float* vecs = reinterpret_cast<const float*>(t_base + ts * L::kTBytes + kImageBytes);
       float ab = vecs[row];                           // a of K S rows, b of Q S rows
       const float cc = lower ? vecs[128 + row] : 0.f;
       const float gamma = vecs[kGamma], bound_a = vecs[kBoundA], bound_u = vecs[kBoundU],
                   bound_s = vecs[kBoundS], image_scale = vecs[lower ? kScaleT : kScalePT];
-      const int64_t t = t0 + (int64_t)ch * kChunk + (row & 63);
-      // 1. K S -> R = V - a K S
-      ok = bar_wait(gbar(g, 3), ph, abort_flag);
-      if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
-      fence_after();
+      ok = __all_sync(0xFFFFFFFFu, bar_wait(gbar(g, 7), ph, abort_flag));
+      if (!ok) break;
       const float smax = __uint_as_float(peak[g][ph][0]), vmax = __uint_as_float(peak[g][ph][1]);
-      // read by all before this step's first product was issued; filled again
-      // after its last one
-      if ((warp & (4 * L::kWG - 1)) == 0 && lane == 0) peak[g][ph ^ 1][0] = peak[g][ph ^ 1][1] = 0;
       const float bound_r = fmaf(bound_a, smax, vmax);
       float scale_r, inv_r, scale_u, inv_u;
       pow2_scale(bound_r, scale_r, inv_r);
       pow2_scale(bound_u * bound_r, scale_u, inv_u);
       ab *= inv_s;
+      // 1. K S -> R = V - a K S
+      ok = bar_wait(gbar(g, 3), ph, abort_flag);
+      if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
+      fence_after();
+      // the other peaks were read before this step's first product, and are
+      // filled again after its last one
+      if ((warp & (4 * L::kWG - 1)) == 0 && lane == 0) peak[g][ph ^ 1][0] = peak[g][ph ^ 1][1] = 0;
       if (lower) {
         const float m = -ab * scale_r;
+        float2 f[4], l[4];
 #pragma unroll
-        for (int c = 0; c < CT; c += 16) {
-          float f[16];
-          product(d1, c, f);
-          const T* ve = reinterpret_cast<const T*>(vr + c / 8);
+        for (int c = 0; c < CT; c += 8) {
+          load2(d1, c, f, l);
+          const uint4 x = load_v(ch, c / 8);
+          const T* ve = reinterpret_cast<const T*>(&x);
+          tmem_ld_wait();
+          add2(f, l);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) f[i] = fmaf(m, f[i], to_f32(ve[i]) * scale_r);
-          store_op(r_op, 64 * 128, row, c, f);
+          for (int i = 0; i < 4; ++i)
+            f[i] = __ffma2_rn(make_float2(m, m), f[i],
+                              __fmul2_rn(make_float2(to_f32(ve[2 * i]), to_f32(ve[2 * i + 1])),
+                                         make_float2(scale_r, scale_r)));
+          store_op(64 * 128, c, f, peak2);
         }
         ready(1);
-        if (ch + 1 < chunks) load_v(ch + 1);
+        if (lane == 0) bar_arrive(t_empty(ts));
+      } else if (lane == 0) {
+        bar_arrive(t_empty(ts));
       }
       // 2. U -> c U, and O = b Q S + P U
       ok = bar_wait(gbar(g, 4), ph, abort_flag);
@@ -862,29 +905,43 @@ delta_chain_kernel(const __grid_constant__ exl3_delta_args a, const uint8_t* __r
       const float from_image = inv_r * image_scale;
       if (lower) {
         const float m = from_image * cc * scale_u;
+        float2 f[4], l[4];
 #pragma unroll
-        for (int c = 0; c < CT; c += 16) {
-          float f[16];
-          product(d2, c, f);
+        for (int c = 0; c < CT; c += 8) {
+          load2(d2, c, f, l);
+          tmem_ld_wait();
+          add2(f, l);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) f[i] *= m;
-          store_op(r_op, 64 * 128, row, c, f);
+          for (int i = 0; i < 4; ++i) f[i] = __fmul2_rn(f[i], make_float2(m, m));
+          store_op(64 * 128, c, f, peak2);
         }
         ready(2);
       } else {
+        const int64_t t = t0 + (int64_t)ch * kChunk + (row & 63);
+        T* o = out + t * a.heads * a.dv;
+        float2 f[4], l[4], p[4], pl[4];
 #pragma unroll
-        for (int c = 0; c < CT; c += 16) {
-          float f[16], p[16];
-          product(d1, c, f);
-          product(d2, c, p);
-          Vec<T, 8> o[2];
+        for (int c = 0; c < CT; c += 8) {
+          load2(d1, c, f, l);
+          load2(d2, c, p, pl);
+          tmem_ld_wait();
+          if (c + 8 == CT) {
+            fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(gbar(g, 2));
+          }
+          add2(f, l);
+          add2(p, pl);
+          Vec<T, 8> y;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i / 8].e[i % 8] = from_f32<T>(fmaf(ab, f[i], from_image * p[i]));
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (t < t1 && col + c + 8 * e < a.dv)
-              *reinterpret_cast<uint4*>(out + t * a.heads * a.dv + c + 8 * e) =
-                  *reinterpret_cast<const uint4*>(&o[e]);
+          for (int i = 0; i < 4; ++i) {
+            const float2 x = __ffma2_rn(make_float2(ab, ab), f[i],
+                                        __fmul2_rn(make_float2(from_image, from_image), p[i]));
+            y.e[2 * i] = from_f32<T>(x.x);
+            y.e[2 * i + 1] = from_f32<T>(x.y);
+          }
+          if (t < t1 && col + c < a.dv)
+            *reinterpret_cast<uint4*>(o + c) = *reinterpret_cast<const uint4*>(&y);
         }
       }
       // 3. the state moves on
@@ -892,151 +949,161 @@ delta_chain_kernel(const __grid_constant__ exl3_delta_args a, const uint8_t* __r
       if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
       fence_after();
 #pragma unroll
-      for (int c = 0; c < CT; c += 16) {
-        float f[16];
-        product(d3, c, f);
+      for (int c = 0; c < CT; c += 8) {
+        float2 f[4], l[4];
+        load2(d3, c, f, l);
+        tmem_ld_wait();
+        add2(f, l);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) S[c + i] = fmaf(gamma, S[c + i], inv_u * f[i]);
+        for (int i = 0; i < 4; ++i)
+          S[c / 2 + i] = __ffma2_rn(make_float2(gamma, gamma), S[c / 2 + i],
+                                    __fmul2_rn(make_float2(inv_u, inv_u), f[i]));
       }
       if (ch + 1 < chunks) {
         pow2_scale(fmaf(bound_s, bound_r, gamma * smax), scale_s, inv_s);
         store_state(scale_s);
-        note_peaks(ch + 1);
         ready(0);
+        // under the next step's first product
+        ok = __all_sync(0xFFFFFFFFu, bar_wait(t_full((ch + 1) % L::kTStages),
+                                              ((ch + 1) / L::kTStages) & 1, abort_flag));
+        if (!ok) break;
+        note_peak_s(ch + 1, __half2float(__hmax(__low2half(peak2), __high2half(peak2))) * inv_s * 1.001f);
+        note_peak_v(ch + 1);
+        __syncwarp();
+        if (lane == 0) bar_arrive(gbar(g, 7));
       }
     }
 #pragma unroll
     for (int c = 0; c < CT; c += 4)
       if (row < a.dk && col + c < a.dv)
         *reinterpret_cast<float4*>(a.state_out + state_at + (int64_t)row * a.dv + col + c) =
-            make_float4(S[c], S[c + 1], S[c + 2], S[c + 3]);
+            make_float4(S[c / 2].x, S[c / 2].y, S[c / 2 + 1].x, S[c / 2 + 1].y);
   } else if (warp < L::kEpiWarps + GROUPS) {
-    // ---------------- products: one thread per group ----------------
-    const int g = warp - L::kEpiWarps;
-    if (lane == 0) {
-      const uint32_t d1 = tmem + (uint32_t)(g * L::kCols), d2 = d1 + 64, d3 = d1 + 128;
-      const uint32_t s_op = smem_u32(s_base + g * L::kSBytes);
-      const uint32_t r_op = smem_u32(r_base + g * L::kRBytes);
-      const int ksteps = (a.dk + 15) / 16;
-      bool ok = true;
-      for (int ch = 0; ch < chunks && ok; ++ch) {
-        const uint32_t ph = ch & 1;
-        const int ks = ch % L::kKQStages, ts = ch % L::kTStages;
-        const uint32_t kq = smem_u32(kq_base + ks * L::kKQ);
-        const uint32_t ti = smem_u32(t_base + ts * kImageBytes);
-        // [K; Q] S
-        ok = bar_wait(kq_full(ks), (ch / L::kKQStages) & 1, abort_flag) &&
-             bar_wait(gbar(g, 0), ph, abort_flag);
-        if (!ok) break;
-        fence_after();
-        for (int k = 0; k < ksteps; ++k) {
-          const uint32_t ao = kq + (k >> 2) * L::kBox + (k & 3) * 32, bo = s_op + k * 2048;
-          mma(d1, desc(ao, 16), desc(bo, 16), idesc(64, false), k > 0);
-          if constexpr (!kPacked) mma(d1, desc(ao, 16), desc(bo + 128 * 128, 16), idesc(64, false), true);
-        }
-        commit(gbar(g, 3));
-        // [T; P T] R
-        ok = bar_wait(t_full(ts), (ch / L::kTStages) & 1, abort_flag) &&
-             bar_wait(gbar(g, 1), ph, abort_flag);
-        if (!ok) break;
-        fence_after();
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t ao = ti + k * 32, bo = r_op + k * 2048;
-          mma(d2, desc(ao, 16), desc(bo, 16), idesc(64, false), k > 0);
-          if constexpr (!kPacked) mma(d2, desc(ao, 16), desc(bo + 64 * 128, 16), idesc(64, false), true);
-          mma(d2, desc(ao + kImageBytes / 2, 16), desc(bo, 16), idesc(NV, false), true);
-        }
-        commit(gbar(g, 4));
-        commit(t_empty(ts));
-        // K^T U
-        ok = bar_wait(gbar(g, 2), ph, abort_flag);
-        if (!ok) break;
-        fence_after();
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t ao = kq + k * 2048, bo = r_op + k * 2048;
-          mma(d3, desc(ao, L::kBox), desc(bo, 16), idesc(64, true), k > 0);
-          if constexpr (!kPacked)
-            mma(d3, desc(ao, L::kBox), desc(bo + 64 * 128, 16), idesc(64, true), true);
-        }
-        commit(gbar(g, 5));
-        commit(kq_empty(ks));
-      }
-      // whatever was issued has finished before tensor memory is freed
-      commit(gbar(g, 6));
-      bar_drain(gbar(g, 6), 0);
-    }
-  } else {
-    // ---------------- producers ----------------
-    const int pt = tid - 32 * (L::kEpiWarps + GROUPS);
-    const int pieces = a.dk / 8;
-    const T* qp = static_cast<const T*>(a.q) + kh * a.q_strides[1];
-    const T* kp = static_cast<const T*>(a.k) + kh * a.k_strides[1];
-    int issued = 0;
+    // ---------------- products: one warp per group ----------------
+    const int g = GROUPS == 1 ? 0 : __shfl_sync(0xFFFFFFFFu, warp - L::kEpiWarps, 0);
+    const uint32_t el = elect_lane();
+    const uint32_t d1 = __shfl_sync(0xFFFFFFFFu, tmem, 0) + (uint32_t)(g * L::kCols), d2 = d1 + 2 * NV,
+                   d3 = d2;
+    const uint32_t bs = desc(smem_u32(op_base + g * L::kOpBytes), 128 * 128);
+    const uint32_t br = desc(smem_u32(op_base + g * L::kOpBytes), 64 * 128);
+    const int ksteps = (a.dk + 15) / 16;
     bool ok = true;
     for (int ch = 0; ch < chunks && ok; ++ch) {
+      const uint32_t ph = ch & 1;
       const int ks = ch % L::kKQStages, ts = ch % L::kTStages;
-      if (pt == 0) {
-        if (ch >= L::kTStages)
-          ok = bar_wait(t_empty(ts), (ch / L::kTStages - 1) & 1, abort_flag);
-        if (ok) {
-          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(t_full(ts)),
-                       "r"(kImageBytes)
-                       : "memory");
-          asm volatile(
-              "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
-                  "r"(smem_u32(t_base + ts * kImageBytes)),
-              "l"(img + ch * img_step), "r"(kImageBytes), "r"(t_full(ts))
-              : "memory");
-          issued = ch + 1;
-        }
-      }
-      if (ok && ch >= L::kKQStages)
-        ok = bar_wait(kq_empty(ks), (ch / L::kKQStages - 1) & 1, abort_flag);
+      const uint32_t kq = desc(smem_u32(kq_base + ks * kKqBytes), 16);
+      const uint32_t kt = desc(smem_u32(kq_base + ks * kKqBytes), L::kBox);
+      const uint32_t ti = desc(smem_u32(t_base + ts * L::kTBytes), 16);
+      // [K; Q] S, both parts
+      ok = bar_wait(kq_full(ks), (ch / L::kKQStages) & 1, abort_flag) &&
+           bar_wait(gbar(g, 0), ph, abort_flag);
       if (!__all_sync(0xFFFFFFFFu, ok)) break;
-      uint8_t* kq = kq_base + ks * L::kKQ;
-      const float* scales = reinterpret_cast<const float*>(img + ch * img_step + kImageBytes) + kRowScale;
+      fence_after();
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (k >= ksteps) break;
+        const uint32_t da = kq + (((k >> 2) * L::kBox + (k & 3) * 32) >> 4), db = bs + (k * 2048 >> 4);
+        if (k == 0)
+          mma<false>(d1, da, db, idesc(2 * NV, false), el);
+        else
+          mma<true>(d1, da, db, idesc(2 * NV, false), el);
+      }
+      commit(gbar(g, 3), el);
+      // [T; P T] R: high with both parts, low with the high one
+      ok = bar_wait(t_full(ts), (ch / L::kTStages) & 1, abort_flag) &&
+           bar_wait(gbar(g, 1), ph, abort_flag);
+      if (!__all_sync(0xFFFFFFFFu, ok)) break;
+      fence_after();
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t da = ti + (k * 32 >> 4), db = br + (k * 2048 >> 4);
+        if (k == 0)
+          mma<false>(d2, da, db, idesc(2 * NV, false), el);
+        else
+          mma<true>(d2, da, db, idesc(2 * NV, false), el);
+        mma<true>(d2, da + (kImageBytes / 2 >> 4), db, idesc(NV, false), el);
+      }
+      commit(gbar(g, 4), el);
+      commit(t_empty(ts), el);
+      // K^T U
+      ok = bar_wait(gbar(g, 2), ph, abort_flag);
+      if (!__all_sync(0xFFFFFFFFu, ok)) break;
+      fence_after();
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t da = kt + (k * 2048 >> 4), db = br + (k * 2048 >> 4);
+        if (k == 0)
+          mma<false>(d3, da, db, idesc(2 * NV, true), el);
+        else
+          mma<true>(d3, da, db, idesc(2 * NV, true), el);
+      }
+      commit(gbar(g, 5), el);
+      commit(kq_empty(ks), el);
+    }
+    // whatever was issued has finished before tensor memory is freed
+    commit(gbar(g, 6), el);
+    bar_drain(gbar(g, 6), 0);
+  } else {
+    // ---------------- copies ----------------
+    const auto expect = [&](uint32_t full, uint32_t bytes) {
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full), "r"(bytes)
+                   : "memory");
+    };
+    const auto copy = [&](uint8_t* dst, const void* src, uint32_t bytes, uint32_t full) {
+      asm volatile(
+          "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+              smem_u32(dst)),
+          "l"(src), "r"(bytes), "r"(full)
+          : "memory");
+    };
+    const T* v = static_cast<const T*>(a.v) + h * a.v_strides[1] + col_base;
+    const int v_cols = col_end - col_base;
+    int kq_issued = 0, t_issued = 0;
+    for (int ch = 0; ch < chunks; ++ch) {
+      const int ks = ch % L::kKQStages, ts = ch % L::kTStages;
+      bool ok = true;
+      if (ch >= L::kKQStages) ok = bar_wait(kq_empty(ks), (ch / L::kKQStages - 1) & 1, abort_flag);
+      if (!__all_sync(0xFFFFFFFFu, ok)) break;
+      if (lane == 0) {
+        expect(kq_full(ks), kKqBytes);
+        copy(kq_base + ks * kKqBytes, kq_img + ch * img_step, kKqBytes, kq_full(ks));
+      }
+      kq_issued = ch + 1;
+      if (ch >= L::kTStages) ok = bar_wait(t_empty(ts), (ch / L::kTStages - 1) & 1, abort_flag);
+      if (!__all_sync(0xFFFFFFFFu, ok)) break;
+      uint8_t* tile = t_base + ts * L::kTBytes;
       const int64_t tc = t0 + (int64_t)ch * kChunk;
       const int n = (int)(t1 - tc < kChunk ? t1 - tc : kChunk);
-      for (int i0 = pt; i0 < 128 * pieces; i0 += 32 * L::kProducers * 4) {
-        uint4 x[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int i = i0 + u * 32 * L::kProducers;
-          const int r = i / pieces, q = i - r * pieces, row = r & 63;
-          x[u] = make_uint4(0, 0, 0, 0);
-          if (r < 128 && row < n)
-            x[u] = r < 64 ? load8(kp + (tc + row) * a.k_strides[0] + 8 * q, vec & 1)
-                          : load8(qp + (tc + row) * a.q_strides[0] + 8 * q, vec & 1);
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int i = i0 + u * 32 * L::kProducers;
-          const int r = i / pieces, q = i - r * pieces;
-          if (r >= 128) break;
-          uint8_t* dst = kq + (q >> 3) * L::kBox + swz(r, q & 7);
-          if constexpr (!std::is_same<T, __half>::value) {
-            const float f = scales[r];
-            const T* e = reinterpret_cast<const T*>(&x[u]);
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const __half2 p = __floats2half2_rn(to_f32(e[2 * j]) * f, to_f32(e[2 * j + 1]) * f);
-              w[j] = *reinterpret_cast<const uint32_t*>(&p);
-            }
-            x[u] = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-          *reinterpret_cast<uint4*>(dst) = x[u];
-        }
+      if (lane == 0) {
+        expect(t_full(ts), kHeadBytes);
+        copy(tile, img + ch * img_step, kHeadBytes, t_full(ts));
       }
-      fence_async();
-      bar_arrive(kq_full(ks));
+      // v in 16-byte pieces; zeros for rows past the sequence, whatever
+      // follows it in memory, and for columns past dv
+      constexpr int kPieces = L::kVRow / 16;
+      for (int i = lane; i < kChunk * kPieces; i += 32) {
+        const int r = i / kPieces, q = i % kPieces;
+        uint8_t* dst = tile + kHeadBytes + r * L::kVRow + ((q ^ (r & kPieces - 1 & 7)) << 4);
+        const bool in = r < n && 8 * q < v_cols;
+        const T* src = v + (tc + (in ? r : 0)) * a.v_strides[0] + (in ? 8 * q : 0);
+        if (vec & 2)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src),
+                       "r"(in ? 16 : 0)
+                       : "memory");
+        else
+          *reinterpret_cast<uint4*>(dst) = in ? load8(src, false) : make_uint4(0, 0, 0, 0);
+      }
+      if (vec & 2)
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(t_full(ts)) : "memory");
+      else
+        bar_arrive(t_full(ts));
+      t_issued = ch + 1;
     }
-    // stopped early: copies in flight land before the CTA exits
-    if (pt == 0 && *abort_flag)
-      for (int ch = issued > L::kTStages ? issued - L::kTStages : 0; ch < issued; ++ch)
-        bar_drain(t_full(ch % L::kTStages), (ch / L::kTStages) & 1);
+    // if the others stopped early: copies in flight land before the CTA exits
+    for (int ch = kq_issued > L::kKQStages ? kq_issued - L::kKQStages : 0; ch < kq_issued; ++ch)
+      bar_drain(kq_full(ch % L::kKQStages), (ch / L::kKQStages) & 1);
+    for (int ch = t_issued > L::kTStages ? t_issued - L::kTStages : 0; ch < t_issued; ++ch)
+      bar_drain(t_full(ch % L::kTStages), (ch / L::kTStages) & 1);
   }
   __syncwarp();
   fence_before();
@@ -1050,7 +1117,7 @@ delta_chain_kernel(const __grid_constant__ exl3_delta_args a, const uint8_t* __r
 
 template <typename T, int GROUPS, int NV, int CT>
 int launch_chain(const exl3_delta_args& a, const uint8_t* ws, int vec, cudaStream_t stream) {
-  using L = Geo<T, GROUPS, NV, CT>;
+  using L = Geo<GROUPS, NV, CT>;
   static DeviceBits attr_done;
   int dev = 0;
   EXL3_CUDA(cudaGetDevice(&dev));
@@ -1095,7 +1162,7 @@ int launch_chunks(const exl3_delta_args& a, uint8_t* ws, cudaStream_t stream) {
 }  // namespace
 
 size_t delta_chunk_ws_bytes(const exl3_delta_args& a) {
-  return (size_t)(a.tokens / kChunk + a.seqs) * a.heads * kSlotBytes;
+  return (size_t)((a.tokens / kChunk + a.seqs) * slot_bytes(a));
 }
 
 int delta_chunks(const exl3_delta_args& a, void* ws, cudaStream_t stream) {
