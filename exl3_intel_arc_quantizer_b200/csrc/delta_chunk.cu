@@ -41,6 +41,7 @@
 // differences behind it exact.
 #include <cuda_bf16.h>
 
+#include <cstddef>
 #include <type_traits>
 
 #include "common.cuh"
@@ -119,55 +120,73 @@ __device__ __forceinline__ uint4 load8(const T* p, bool vec) {
 // ---------------------------------------------------------------------------
 
 constexpr int kPrepThreads = 256;
-constexpr int kLdk = 136;  // elements per row of the staged q and k (17 x 16 bytes)
-constexpr int kLds = 68;   // floats per row of the 64 x 64 matrices
-constexpr int kLdd = 65;
+constexpr int kPrepHeads = 8;  // heads whose gates are prepared at once
+constexpr int kLds = 68;       // floats per row of the 64 x 64 matrices
 
-struct PrepSmem {
-  union {
-    uint16_t kq[2][kChunk][kLdk];
-    struct {
-      float M[kChunk][kLds];
-      float X[kChunk][kLds];
-    } m;
-  } u;
-  float dot[2][kChunk][kLdd];  // k_i . k_j and q_i . k_j, j <= i
-  float P[kChunk][kLds];
-  float tmp[32][36];
-  double G[kChunk];
-  float beta[kChunk], rk[kChunk], rq[kChunk];
-  float rowscale[2 * kChunk];   // power of two that brings a k or q row into fp16
-  uint32_t peak[3];             // bits of max |T|, max |P T|, largest row sum of |T|
+// What depends on a head's g and beta. R_b is the prefix sum before block b
+// of 16 tokens (base 2): for i in block b and j in an earlier one,
+// e^{G_i - G_j} = up[i] down[b - 1][j], both factors <= 1.
+struct alignas(16) Gates {
+  float2 g[kChunk];          // G_i / ln 2 in two parts
+  float up[kChunk];          // 2^(G_i - R_b)
+  float down[3][48];         // 2^(R_b - G_j), b = 1..3, j < 16 b
+  float beta[kChunk];
+  float total[2];            // G_63 / ln 2 in two parts
 };
 
-template <typename T>
+struct PrepSmem {
+  uint8_t kq[kKqBytes];      // the chain's [K; Q]; later P T's two parts
+  union {
+    float M[kChunk][kLds];
+    uint8_t t[2][kChunk * 128];  // T's two parts, when M has been used
+  } m;
+  float X[kChunk][kLds];
+  float tmp[32][36];
+  Gates gates[kPrepHeads];
+  // of row i: the power of two on its way to fp16 and back, and the factor
+  // 1 / |.| (1 where rows are taken as they are)
+  float back[2 * kChunk], unit[2 * kChunk], norm[kChunk];
+  uint32_t peak[3];          // bits of max |T|, max |P T|, largest row sum of |T|
+};
+
+static_assert(sizeof(Gates) % 16 == 0 && offsetof(Gates, g) % 16 == 0 && offsetof(Gates, beta) % 16 == 0 &&
+                  offsetof(PrepSmem, m) % 16 == 0 && offsetof(PrepSmem, X) % 16 == 0 &&
+                  offsetof(PrepSmem, tmp) % 16 == 0 &&
+                  offsetof(PrepSmem, gates) % 16 == 0 && offsetof(PrepSmem, back) % 16 == 0 &&
+                  kLds % 4 == 0,
+              "16-byte accesses");
+
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                          uint32_t b1) {
-  if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
 }
-
+__device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// One CTA per chunk and key head. Bound by instruction issue and the latency
+// of the inverse's steps (two CTAs share an SM); the reads and writes are
+// 64 KB per key head and 33 KB per head.
 template <typename T>
-__global__ void __launch_bounds__(kPrepThreads)
+__global__ void __launch_bounds__(kPrepThreads, 2)
 delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict__ ws, int vec) {
-  extern __shared__ __align__(16) uint8_t dsm[];
-  PrepSmem& sm = *reinterpret_cast<PrepSmem*>(dsm);
+  extern __shared__ __align__(128) uint8_t prep_smem[];
+  PrepSmem& sm = *reinterpret_cast<PrepSmem*>(prep_smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t slot = blockIdx.x;
   const int kh = blockIdx.y;
@@ -185,149 +204,216 @@ delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict
   t0 += (slot - slot_base(t0, s)) * kChunk;
   if (t0 >= t1) return;
   const int n = (int)(t1 - t0 < kChunk ? t1 - t0 : kChunk);
+  uint8_t* const out = ws + slot * slot_bytes(a);
 
-  // q and k of the chunk, zeros past its end and up to a multiple of 16
-  const int pieces = a.dk / 8, padded = (a.dk + 15) / 16 * 2;
-  for (int i = tid; i < 2 * kChunk * padded; i += kPrepThreads) {
-    const int r = i / padded, q = i - r * padded, row = r & (kChunk - 1), isq = r >> 6;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (row < n && q < pieces) {
-      const int64_t* st = isq ? a.q_strides : a.k_strides;
-      v = load8(static_cast<const T*>(isq ? a.q : a.k) + (t0 + row) * st[0] + kh * st[1] + 8 * q, vec);
+  // [K; Q] in fp16, zeros past the chunk's end and past dk: 16 neighbouring
+  // threads hold a row, a thread one 16-byte piece of eight rows
+  {
+    const int q = tid & 15;
+    uint4 x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = (tid >> 4) + 16 * i, row = r & 63;
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (row < n && 8 * q < a.dk)
+        x[i] = i < 4 ? load8(static_cast<const T*>(a.k) + (t0 + row) * a.k_strides[0] + kh * a.k_strides[1] + 8 * q, vec)
+                     : load8(static_cast<const T*>(a.q) + (t0 + row) * a.q_strides[0] + kh * a.q_strides[1] + 8 * q, vec);
     }
-    *reinterpret_cast<uint4*>(&sm.u.kq[isq][row][8 * q]) = v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = (tid >> 4) + 16 * i;
+      const T* e = reinterpret_cast<const T*>(&x[i]);
+      float f[8], ss = 0.f, back = 1.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = to_f32(e[j]);
+      if constexpr (!std::is_same<T, __half>::value) {
+        // the row's largest element goes to [1, 2)
+        float big = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(f[j]));
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
+        uint32_t ex = (__float_as_uint(big) >> 23) & 255u;
+        ex = big == 0.f ? 127u : ex < 2u ? 2u : ex > 252u ? 252u : ex;
+        const float scale = __uint_as_float((254u - ex) << 23);
+        back = __uint_as_float(ex << 23);
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f[2 * j] *= scale;
+          f[2 * j + 1] *= scale;
+          const __half2 p = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
+          w[j] = *reinterpret_cast<const uint32_t*>(&p);
+        }
+        x[i] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      const uint32_t at = (q >> 3) * (kKqBytes / 2) + swz(r, q & 7);
+      *reinterpret_cast<uint4*>(sm.kq + at) = x[i];
+      *reinterpret_cast<uint4*>(out + (int64_t)kh * kKqBytes + at) = x[i];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = fmaf(f[j], f[j], ss);
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+      if (q == 0) {
+        sm.back[r] = back;
+        // 1 / sqrt(|x|^2 + eps) with x = back times what was summed
+        sm.unit[r] = a.normalize_qk ? rsqrtf(fmaf(ss * back, back, kNormEps)) : 1.f;
+        if (i < 4) sm.norm[r] = sqrtf(ss) * back;
+      }
+    }
   }
   __syncthreads();
 
-  // warps 0-3: rows 16 w of K K^T; warps 4-7: of Q K^T; columns up to the
-  // diagonal tile
+  // warps 0-3: rows 16 mt of K K^T; warps 4-7: of Q K^T; columns up to the
+  // diagonal tile. They stay in registers for all heads.
+  const int mt = warp & 3, which = warp >> 2;
+  float acc[8][4];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
   {
-    const int mt = warp & 3, which = warp >> 2;
-    float acc[8][4];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
-    for (int k0 = 0; k0 < a.dk; k0 += 16) {
+    const auto at = [&](int r, int piece) {
+      return smem_u32(sm.kq + (piece >> 3) * (kKqBytes / 2) + swz(r, piece & 7));
+    };
+    for (int k = 0; k < (a.dk + 15) / 16; ++k) {
       uint32_t fa[4];
-      ldsm4(fa, smem_u32(&sm.u.kq[which][16 * mt + (lane & 15)][k0 + 8 * (lane >> 4)]));
+      ldsm4(fa, at(64 * which + 16 * mt + (lane & 15), 2 * k + (lane >> 4)));
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (j > mt) break;
         uint32_t fb[4];  // columns 16 j .. 16 j + 15: two n-tiles, two k halves
-        ldsm4(fb, smem_u32(&sm.u.kq[0][16 * j + (lane & 7) + 8 * (lane >> 4)]
-                                   [k0 + 8 * ((lane >> 3) & 1)]));
-        mma16816<T>(acc[2 * j], fa, fb[0], fb[1]);
-        mma16816<T>(acc[2 * j + 1], fa, fb[2], fb[3]);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (j > 2 * mt + 1) break;
-      const int r = 16 * mt + (lane >> 2), c = 8 * j + 2 * (lane & 3);
-      sm.dot[which][r][c] = acc[j][0];
-      sm.dot[which][r][c + 1] = acc[j][1];
-      sm.dot[which][r + 8][c] = acc[j][2];
-      sm.dot[which][r + 8][c + 1] = acc[j][3];
-    }
-    // |q|^2, and the largest |k| and |q|: four threads per row
-    const int row = tid >> 2;
-    float ss = 0.f, big[2] = {0.f, 0.f};
-    for (int c = tid & 3; c < a.dk; c += 4) {
-      const uint16_t bk = sm.u.kq[0][row][c], bq = sm.u.kq[1][row][c];
-      const float v = to_f32(*reinterpret_cast<const T*>(&bq));
-      ss = fmaf(v, v, ss);
-      big[0] = fmaxf(big[0], fabsf(to_f32(*reinterpret_cast<const T*>(&bk))));
-      big[1] = fmaxf(big[1], fabsf(v));
-    }
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-      big[0] = fmaxf(big[0], __shfl_xor_sync(0xFFFFFFFFu, big[0], o));
-      big[1] = fmaxf(big[1], __shfl_xor_sync(0xFFFFFFFFu, big[1], o));
-    }
-    if ((tid & 3) == 0) {
-      sm.rq[row] = a.normalize_qk ? rsqrtf(ss + kNormEps) : 1.f;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        // the row's largest element goes to [1, 2); fp16 rows stay
-        uint32_t e = (__float_as_uint(big[i]) >> 23) & 255u;
-        e = e < 2u ? 2u : e > 252u ? 252u : e;
-        sm.rowscale[64 * i + row] =
-            std::is_same<T, __half>::value || big[i] == 0.f ? 1.f : __uint_as_float((254u - e) << 23);
+        ldsm4(fb, at(16 * j + (lane & 7) + 8 * (lane >> 4), 2 * k + ((lane >> 3) & 1)));
+        mma16816(acc[2 * j], fa, fb[0], fb[1]);
+        mma16816(acc[2 * j + 1], fa, fb[2], fb[3]);
       }
     }
   }
-  __syncthreads();
-  // [K; Q] as the chain's operand, zeros up to the tiles' ends
-  {
-    uint8_t* dst = ws + slot * slot_bytes(a) + (int64_t)kh * kKqBytes;
-    for (int i = tid; i < 128 * 16; i += kPrepThreads) {
-      const int r = i >> 4, q = i & 15;
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (q < pieces) {
-        x = *reinterpret_cast<const uint4*>(&sm.u.kq[r >> 6][r & 63][8 * q]);
-        if constexpr (!std::is_same<T, __half>::value) {
-          const float f = sm.rowscale[r];
-          const T* e = reinterpret_cast<const T*>(&x);
-          uint32_t w[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const __half2 p = __floats2half2_rn(to_f32(e[2 * j]) * f, to_f32(e[2 * j + 1]) * f);
-            w[j] = *reinterpret_cast<const uint32_t*>(&p);
-          }
-          x = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      }
-      *reinterpret_cast<uint4*>(dst + (q >> 3) * (kKqBytes / 2) + swz(r, q & 7)) = x;
-    }
-  }
-  if (tid < kChunk) sm.rk[tid] = a.normalize_qk ? rsqrtf(sm.dot[0][tid][tid] + kNormEps) : 1.f;
-  float knorm[2] = {0.f, 0.f};  // |k| of rows 2 lane and 2 lane + 1
-  if (warp == 0) {
-    knorm[0] = sqrtf(sm.dot[0][2 * lane][2 * lane]);
-    knorm[1] = sqrtf(sm.dot[0][2 * lane + 1][2 * lane + 1]);
-  }
+  const int r0 = 16 * mt + (lane >> 2), c0 = 2 * (lane & 3);  // of a fragment's first element
 
   const int rep = a.heads / a.key_heads;
-  for (int h = kh * rep; h < (kh + 1) * rep; ++h) {
-    __syncthreads();  // rk, and the last head's matrices read
+  for (int h = 0; h < rep; ++h) {
+    const int head = kh * rep + h;
+    uint8_t* const img = out + (int64_t)a.key_heads * kKqBytes + head * kHeadBytes;
+    float* const vecs = reinterpret_cast<float*>(img + kImageBytes);
+    if (h % kPrepHeads == 0) {
+      if (h) __syncthreads();
+      if (h + warp < rep) {
+        // a warp per head: prefix sums in fp64
+        Gates& gt = sm.gates[warp];
+        double g[2], run;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = 2 * lane + i;
+          float v = r < n ? a.g[(t0 + r) * a.g_stride + head + warp] : 0.f;
+          v = v < -200.f ? -200.f : v;
+          g[i] = (double)v * 1.4426950408889634;  // base 2
+          gt.beta[r] = r < n ? a.beta[(t0 + r) * a.beta_stride + head + warp] : 0.f;
+        }
+        run = g[0] + g[1];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double up = __shfl_up_sync(0xFFFFFFFFu, run, o);
+          if (lane >= o) run += up;
+        }
+        const double G[2] = {run - g[1], run};
+        const double before = __shfl_sync(0xFFFFFFFFu, run, (lane & ~7) - 1);  // R of this block
+        const double R = lane < 8 ? 0.0 : before;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = 2 * lane + i;
+          const float hi = (float)G[i];
+          gt.g[r] = make_float2(hi, (float)(G[i] - (double)hi));
+          gt.up[r] = exp2_fast((float)(G[i] - R));
+        }
+#pragma unroll
+        for (int b = 1; b < 4; ++b) {
+          const double Rb = __shfl_sync(0xFFFFFFFFu, run, 8 * b - 1);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (2 * lane + i < 16 * b) gt.down[b - 1][2 * lane + i] = exp2_fast((float)(Rb - G[i]));
+        }
+        if (lane == 31) {
+          const float hi = (float)run;
+          gt.total[0] = hi;
+          gt.total[1] = (float)(run - (double)hi);
+        }
+      }
+      __syncthreads();
+    }
+    const Gates& gt = sm.gates[h % kPrepHeads];
     if (tid < 3) sm.peak[tid] = 0;
-    if (warp == 0) {
-      double g[2], run;
+
+    // M into shared memory; P as the first operand of P T, in two fp16 parts
+    // under the warp's scale
+    uint32_t ph[4][4], pl[4][4];
+    float inv_p = 1.f;
+    {
+      float f[8][4];
+      float row[2], up[2];
+      float2 gr[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int r = 2 * lane + i;
-        float v = r < n ? a.g[(t0 + r) * a.g_stride + h] : 0.f;
-        v = v < -200.f ? -200.f : v;
-        g[i] = (double)v;
-        sm.beta[r] = r < n ? a.beta[(t0 + r) * a.beta_stride + h] : 0.f;
+        const int r = r0 + 8 * i;
+        row[i] = which ? a.scale * sm.unit[64 + r] * sm.back[64 + r] : gt.beta[r] * sm.unit[r] * sm.back[r];
+        up[i] = row[i] * gt.up[r];
+        gr[i] = gt.g[r];
       }
-      run = g[0] + g[1];
+      float most = 0.f;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double up = __shfl_up_sync(0xFFFFFFFFu, run, o);
-        if (lane >= o) run += up;
+      for (int j = 0; j < 8; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[j][e] = 0.f;
+        if (j > 2 * mt + 1) continue;
+        const int c = 8 * j + c0;
+        const float2 u = *reinterpret_cast<const float2*>(&sm.unit[c]);
+        const float2 bk = *reinterpret_cast<const float2*>(&sm.back[c]);
+        float2 col = make_float2(u.x * bk.x, u.y * bk.y);
+        if (j < 2 * mt) {
+          const float2 dn = *reinterpret_cast<const float2*>(&gt.down[mt - 1][c]);
+          col.x *= dn.x;
+          col.y *= dn.y;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            f[j][2 * i] = acc[j][2 * i] * col.x * up[i];
+            f[j][2 * i + 1] = acc[j][2 * i + 1] * col.y * up[i];
+          }
+        } else {
+          const float4 gc = *reinterpret_cast<const float4*>(&gt.g[c]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int r = r0 + 8 * i;
+            const float d0 = exp2_fast((gr[i].x - gc.x) + (gr[i].y - gc.y));
+            const float d1 = exp2_fast((gr[i].x - gc.z) + (gr[i].y - gc.w));
+            const int last = which ? r : r - 1;  // P has its diagonal
+            f[j][2 * i] = c <= last ? acc[j][2 * i] * col.x * row[i] * d0 : 0.f;
+            f[j][2 * i + 1] = c + 1 <= last ? acc[j][2 * i + 1] * col.y * row[i] * d1 : 0.f;
+          }
+        }
+        if (which) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(f[j][e]));
+        } else {
+          *reinterpret_cast<float2*>(&sm.m.M[r0][c]) = make_float2(f[j][0], f[j][1]);
+          *reinterpret_cast<float2*>(&sm.m.M[r0 + 8][c]) = make_float2(f[j][2], f[j][3]);
+        }
       }
-      sm.G[2 * lane] = run - g[1];
-      sm.G[2 * lane + 1] = run;
+      if (which) {
+        most = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most)));
+        float scale;
+        pow2_scale(most, scale, inv_p);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float* v = &f[2 * k + (e >> 1)][2 * (e & 1)];
+            split2(make_float2(v[0] * scale, v[1] * scale), ph[k][e], pl[k][e]);
+          }
+      }
     }
     __syncthreads();
-    float(&M)[kChunk][kLds] = sm.u.m.M;
-    float(&X)[kChunk][kLds] = sm.u.m.X;
-    for (int i = tid; i < kChunk * kChunk; i += kPrepThreads) {
-      const int r = i >> 6, c = i & 63;
-      float m = 0.f, p = 0.f;
-      if (c <= r) {
-        const float d = expf((float)(sm.G[r] - sm.G[c])) * sm.rk[c];
-        p = a.scale * sm.rq[r] * d * sm.dot[1][r][c];
-        if (c < r) m = sm.beta[r] * sm.rk[r] * d * sm.dot[0][r][c];
-      }
-      M[r][c] = m;
-      sm.P[r][c] = p;
-      X[r][c] = 0.f;
-    }
-    __syncthreads();
+    float(&M)[kChunk][kLds] = sm.m.M;
+    float(&X)[kChunk][kLds] = sm.X;
     // (I + M)^-1: the 16x16 diagonal blocks, a thread per column
     if (tid < 64) {
       const int b = tid & ~15, c = tid & 15;
@@ -336,7 +422,13 @@ delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict
       for (int i = 0; i < 16; ++i) {
         float v = i == c ? 1.f : 0.f;
 #pragma unroll
-        for (int j = 0; j < i; ++j) v = fmaf(-M[b + i][b + j], x[j], v);
+        for (int j = 0; j < i; j += 4) {
+          const float4 m = *reinterpret_cast<const float4*>(&M[b + i][b + j]);
+          v = fmaf(-m.x, x[j], v);
+          if (j + 1 < i) v = fmaf(-m.y, x[j + 1], v);
+          if (j + 2 < i) v = fmaf(-m.z, x[j + 2], v);
+          if (j + 3 < i) v = fmaf(-m.w, x[j + 3], v);
+        }
         x[i] = v;
       }
 #pragma unroll
@@ -346,157 +438,172 @@ delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict
     // halves of 32: X21 = -X22 (M21 X11), two pairs of blocks at once
     {
       const int p = tid >> 7, r = (tid >> 3) & 15, c = 2 * (tid & 7), b = 32 * p;
-      float v0 = 0.f, v1 = 0.f;
+      float2 v = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const float m = M[b + 16 + r][b + k];
-        v0 = fmaf(m, X[b + k][b + c], v0);
-        v1 = fmaf(m, X[b + k][b + c + 1], v1);
+      for (int k = 0; k < 16; k += 4) {
+        const float4 m = *reinterpret_cast<const float4*>(&M[b + 16 + r][b + k]);
+        v = __ffma2_rn(make_float2(m.x, m.x), *reinterpret_cast<const float2*>(&X[b + k][b + c]), v);
+        v = __ffma2_rn(make_float2(m.y, m.y), *reinterpret_cast<const float2*>(&X[b + k + 1][b + c]), v);
+        v = __ffma2_rn(make_float2(m.z, m.z), *reinterpret_cast<const float2*>(&X[b + k + 2][b + c]), v);
+        v = __ffma2_rn(make_float2(m.w, m.w), *reinterpret_cast<const float2*>(&X[b + k + 3][b + c]), v);
       }
-      sm.tmp[16 * p + r][c] = v0;
-      sm.tmp[16 * p + r][c + 1] = v1;
+      *reinterpret_cast<float2*>(&sm.tmp[16 * p + r][c]) = v;
       __syncthreads();
-      v0 = v1 = 0.f;
+      v = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const float m = X[b + 16 + r][b + 16 + k];
-        v0 = fmaf(m, sm.tmp[16 * p + k][c], v0);
-        v1 = fmaf(m, sm.tmp[16 * p + k][c + 1], v1);
+      for (int k = 0; k < 16; k += 4) {
+        const float4 m = *reinterpret_cast<const float4*>(&X[b + 16 + r][b + 16 + k]);
+        const float* w = &sm.tmp[16 * p + k][c];
+        v = __ffma2_rn(make_float2(m.x, m.x), *reinterpret_cast<const float2*>(w), v);
+        v = __ffma2_rn(make_float2(m.y, m.y), *reinterpret_cast<const float2*>(w + 36), v);
+        v = __ffma2_rn(make_float2(m.z, m.z), *reinterpret_cast<const float2*>(w + 72), v);
+        v = __ffma2_rn(make_float2(m.w, m.w), *reinterpret_cast<const float2*>(w + 108), v);
       }
-      X[b + 16 + r][b + c] = -v0;
-      X[b + 16 + r][b + c + 1] = -v1;
+      *reinterpret_cast<float2*>(&X[b + 16 + r][b + c]) = make_float2(-v.x, -v.y);
+      // the blocks above the diagonal of X11 and X22
+      *reinterpret_cast<float2*>(&X[b + r][b + 16 + c]) = make_float2(0.f, 0.f);
     }
     __syncthreads();
     // the whole: the same with blocks of 32
     {
       const int r = tid >> 3, c = 4 * (tid & 7);
-      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      float2 v[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      const auto product = [&](const float* left, const float* right, int pitch) {
 #pragma unroll
-      for (int k = 0; k < 32; ++k) {
-        const float m = M[32 + r][k];
-        const float4 x = *reinterpret_cast<const float4*>(&X[k][c]);
-        v[0] = fmaf(m, x.x, v[0]);
-        v[1] = fmaf(m, x.y, v[1]);
-        v[2] = fmaf(m, x.z, v[2]);
-        v[3] = fmaf(m, x.w, v[3]);
-      }
-      *reinterpret_cast<float4*>(&sm.tmp[r][c]) = make_float4(v[0], v[1], v[2], v[3]);
-      __syncthreads();
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = 0.f;
-#pragma unroll
-      for (int k = 0; k < 32; ++k) {
-        const float m = X[32 + r][32 + k];
-        const float4 x = *reinterpret_cast<const float4*>(&sm.tmp[k][c]);
-        v[0] = fmaf(m, x.x, v[0]);
-        v[1] = fmaf(m, x.y, v[1]);
-        v[2] = fmaf(m, x.z, v[2]);
-        v[3] = fmaf(m, x.w, v[3]);
-      }
-      *reinterpret_cast<float4*>(&X[32 + r][c]) = make_float4(-v[0], -v[1], -v[2], -v[3]);
-    }
-    __syncthreads();
-    // T = X beta into M's place, P T into tmp-free registers: a 4x4 tile each
-    uint8_t* img = ws + slot * slot_bytes(a) + (int64_t)a.key_heads * kKqBytes + h * kHeadBytes;
-    {
-      const int r = 4 * (tid >> 4), c = 4 * (tid & 15);
-      float v[4][4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[i][e] = 0.f;
-      if (c <= r) {
-        for (int k = c; k < r + 4; k += 4) {  // P is zero past the diagonal, X before it
-          float p[4][4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float4 t = *reinterpret_cast<const float4*>(&sm.P[r + i][k]);
-            p[i][0] = t.x;
-            p[i][1] = t.y;
-            p[i][2] = t.z;
-            p[i][3] = t.w;
-          }
+        for (int k = 0; k < 32; k += 4) {
+          const float4 m = *reinterpret_cast<const float4*>(left + k);
+          const float w[4] = {m.x, m.y, m.z, m.w};
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {
-            const float4 x = *reinterpret_cast<const float4*>(&X[k + kk][c]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              v[i][0] = fmaf(p[i][kk], x.x, v[i][0]);
-              v[i][1] = fmaf(p[i][kk], x.y, v[i][1]);
-              v[i][2] = fmaf(p[i][kk], x.z, v[i][2]);
-              v[i][3] = fmaf(p[i][kk], x.w, v[i][3]);
-            }
+            const float4 x = *reinterpret_cast<const float4*>(right + (k + kk) * pitch);
+            v[0] = __ffma2_rn(make_float2(w[kk], w[kk]), make_float2(x.x, x.y), v[0]);
+            v[1] = __ffma2_rn(make_float2(w[kk], w[kk]), make_float2(x.z, x.w), v[1]);
           }
         }
-      }
-      const float4 bt = *reinterpret_cast<const float4*>(&sm.beta[c]);
-      float x[4][4];
-      float most = 0.f, most_p = 0.f, sum = 0.f;
+      };
+      product(&M[32 + r][0], &X[0][c], kLds);
+      *reinterpret_cast<float4*>(&sm.tmp[r][c]) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+      __syncthreads();
+      v[0] = v[1] = make_float2(0.f, 0.f);
+      product(&X[32 + r][32], &sm.tmp[0][c], 36);
+      *reinterpret_cast<float4*>(&X[32 + r][c]) = make_float4(-v[0].x, -v[0].y, -v[1].x, -v[1].y);
+    }
+    __syncthreads();
+    // T = X beta: 16 columns of a row per thread, its peak and row sums
+    {
+      const int r = tid >> 2, c = 16 * (tid & 3);
+      float2 x[8];
+      float most = 0.f, sum = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float4 t = *reinterpret_cast<const float4*>(&X[r + i][c]);
-        x[i][0] = t.x * bt.x;
-        x[i][1] = t.y * bt.y;
-        x[i][2] = t.z * bt.z;
-        x[i][3] = t.w * bt.w;
-        v[i][0] *= bt.x;
-        v[i][1] *= bt.y;
-        v[i][2] *= bt.z;
-        v[i][3] *= bt.w;
-        float row = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          row += fabsf(x[i][e]);
-          most = fmaxf(most, fabsf(x[i][e]));
-          most_p = fmaxf(most_p, fabsf(v[i][e]));
+        float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+        // X is written up to its 32-blocks; beyond the row's diagonal is zero
+        if (c + 4 * i <= r) {
+          t = *reinterpret_cast<const float4*>(&X[r][c + 4 * i]);
+          const float4 b = *reinterpret_cast<const float4*>(&gt.beta[c + 4 * i]);
+          t = make_float4(t.x * b.x, t.y * b.y, t.z * b.z, t.w * b.w);
         }
-        // the row's 16 threads are neighbours
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) row += __shfl_xor_sync(0xFFFFFFFFu, row, o);
-        sum = fmaxf(sum, row);
+        x[2 * i] = make_float2(t.x, t.y);
+        x[2 * i + 1] = make_float2(t.z, t.w);
+        sum += (fabsf(t.x) + fabsf(t.y)) + (fabsf(t.z) + fabsf(t.w));
+        most = fmaxf(fmaxf(most, fmaxf(fabsf(t.x), fabsf(t.y))), fmaxf(fabsf(t.z), fabsf(t.w)));
       }
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
       // the order of these maxima (of bits of non-negative floats) does not matter
       const uint32_t m0 = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most));
-      const uint32_t m1 = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most_p));
       const uint32_t m2 = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(sum));
       if (lane == 0) {
         atomicMax(&sm.peak[0], m0);
-        atomicMax(&sm.peak[1], m1);
         atomicMax(&sm.peak[2], m2);
       }
       __syncthreads();
-      float st, sp, inv;
-      pow2_scale(__uint_as_float(sm.peak[0]), st, inv);
-      pow2_scale(__uint_as_float(sm.peak[1]), sp, inv);
+      float scale, inv;
+      pow2_scale(__uint_as_float(sm.peak[0]), scale, inv);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint2 hi, lo;
-        split2(make_float2(x[i][0] * st, x[i][1] * st), hi.x, lo.x);
-        split2(make_float2(x[i][2] * st, x[i][3] * st), hi.y, lo.y);
-        const uint32_t at = swz(r + i, c >> 3) + 2 * (c & 7);
-        *reinterpret_cast<uint2*>(img + at) = hi;
-        *reinterpret_cast<uint2*>(img + kImageBytes / 2 + at) = lo;
-        split2(make_float2(v[i][0] * sp, v[i][1] * sp), hi.x, lo.x);
-        split2(make_float2(v[i][2] * sp, v[i][3] * sp), hi.y, lo.y);
-        const uint32_t at2 = swz(64 + r + i, c >> 3) + 2 * (c & 7);
-        *reinterpret_cast<uint2*>(img + at2) = hi;
-        *reinterpret_cast<uint2*>(img + kImageBytes / 2 + at2) = lo;
+      for (int e = 0; e < 2; ++e) {
+        uint4 hi, lo;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[4 * e + i] = __fmul2_rn(x[4 * e + i], make_float2(scale, scale));
+        split8(x + 4 * e, hi, lo);
+        const uint32_t at = swz(r, c / 8 + e);
+        *reinterpret_cast<uint4*>(sm.m.t[0] + at) = hi;
+        *reinterpret_cast<uint4*>(sm.m.t[1] + at) = lo;
+        *reinterpret_cast<uint4*>(img + at) = hi;
+        *reinterpret_cast<uint4*>(img + kImageBytes / 2 + at) = lo;
       }
     }
-    float* vout = reinterpret_cast<float*>(img + kImageBytes);
-    if (warp == 0) {
+    __syncthreads();
+    if (which) {
+      // P T, rows of this warp: three products of parts per 16 x 16 block
+      float o[8][4];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (k > mt) break;
+#pragma unroll
+        for (int j = 0; j <= k; ++j) {
+          const uint32_t at = swz(16 * k + (lane & 15), 2 * j + (lane >> 4));
+          uint32_t bh[4], bl[4];
+          ldsm4_trans(bh, smem_u32(sm.m.t[0] + at));
+          ldsm4_trans(bl, smem_u32(sm.m.t[1] + at));
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            mma16816(o[2 * j + e], ph[k], bh[2 * e], bh[2 * e + 1]);
+            mma16816(o[2 * j + e], ph[k], bl[2 * e], bl[2 * e + 1]);
+            mma16816(o[2 * j + e], pl[k], bh[2 * e], bh[2 * e + 1]);
+          }
+        }
+      }
+      float scale, inv, most = 0.f;
+      pow2_scale(__uint_as_float(sm.peak[0]), scale, inv);
+      inv *= inv_p;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          o[j][e] *= inv;
+          most = fmaxf(most, fabsf(o[j][e]));
+        }
+      const uint32_t m1 = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most));
+      if (lane == 0) atomicMax(&sm.peak[1], m1);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      pow2_scale(__uint_as_float(sm.peak[1]), scale, inv);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t hi, lo;
+          split2(make_float2(o[j][2 * i] * scale, o[j][2 * i + 1] * scale), hi, lo);
+          const uint32_t at = swz(r0 + 8 * i, j) + 2 * c0;
+          *reinterpret_cast<uint32_t*>(sm.kq + at) = hi;
+          *reinterpret_cast<uint32_t*>(sm.kq + kChunk * 128 + at) = lo;
+        }
+      if (tid == 128) vecs[kScalePT] = inv;
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      // rows 64-127 of the image's two tiles
+      for (int i = tid - 128; i < 2 * kChunk * 8; i += 128) {
+        const int part = i >> 9, at = (i & 511) * 16;
+        *reinterpret_cast<uint4*>(img + part * (kImageBytes / 2) + kChunk * 128 + at) =
+            *reinterpret_cast<const uint4*>(sm.kq + part * (kChunk * 128) + at);
+      }
+    } else if (warp == 0) {
       float ba = 0.f, bu = 0.f, bs = 0.f;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int r = 2 * lane + i;
-        const float up = 1.f / sm.rowscale[r], eg = expf((float)sm.G[r]);
-        const float c = sm.rk[r] * expf((float)(sm.G[63] - sm.G[r]));
-        vout[r] = eg * sm.rk[r] * up;
-        vout[64 + r] = a.scale * sm.rq[r] * eg / sm.rowscale[64 + r];
-        vout[128 + r] = c * up;
-        ba = fmaxf(ba, eg * sm.rk[r] * knorm[i]);
-        bu = fmaxf(bu, c * up);
-        bs += c * knorm[i];
+        const float2 g = gt.g[r];
+        const float eg = exp2_fast(g.x + g.y) * sm.unit[r];
+        const float c = exp2_fast((gt.total[0] - g.x) + (gt.total[1] - g.y)) * sm.unit[r];
+        vecs[r] = eg * sm.back[r];
+        vecs[64 + r] = a.scale * exp2_fast(g.x + g.y) * sm.unit[64 + r] * sm.back[64 + r];
+        vecs[128 + r] = c * sm.back[r];
+        ba = fmaxf(ba, eg * sm.norm[r]);
+        bu = fmaxf(bu, c * sm.back[r]);
+        bs += c * sm.norm[r];
       }
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -507,16 +614,15 @@ delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict
       if (lane == 0) {
         const float t = __uint_as_float(sm.peak[2]);
         float scale, inv;
-        vout[kGamma] = expf((float)sm.G[63]);
-        vout[kBoundA] = ba * sqrtf((float)a.dk);
-        vout[kBoundU] = bu * t;
-        vout[kBoundS] = bs * t;
         pow2_scale(__uint_as_float(sm.peak[0]), scale, inv);
-        vout[kScaleT] = inv;
-        pow2_scale(__uint_as_float(sm.peak[1]), scale, inv);
-        vout[kScalePT] = inv;
+        vecs[kGamma] = exp2_fast(gt.total[0] + gt.total[1]);
+        vecs[kBoundA] = ba * sqrtf((float)a.dk) * 1.001f;
+        vecs[kBoundU] = bu * t;
+        vecs[kBoundS] = bs * t;
+        vecs[kScaleT] = inv;
       }
     }
+    if (h + 1 < rep) __syncthreads();  // T's place is M's again
   }
 }
 
