@@ -8,20 +8,23 @@
 //
 // The second norm takes h before its rounding. Bound: HBM, each tensor moved
 // once: a row stays in registers as fp32 between its two sums. Rows of up to
-// 1,024 elements belong to part of a warp or a warp (sums by shuffles), longer
-// ones to a CTA (one barrier per sum); rows past the registers of a CTA are
-// read again for each sum.
+// 128 vectors belong to part of a warp or a warp (sums by shuffles), longer
+// ones to a CTA (one barrier per sum). CTAs walk over the rows and load the
+// next row's vectors before they work on this one's, so that loads are in
+// flight across the sums; rows past the registers of a CTA are read again for
+// each sum.
 #include "common.cuh"
 #include "vec_types.cuh"
 
 namespace exl3 {
 namespace {
 
-constexpr int kMaxThreads = 512;  // of a CTA that owns a row: 128 registers each
+constexpr int kMaxThreads = 512;  // of a CTA that owns a row
 
 __device__ __forceinline__ float act_sigmoid(float z) {
-  // exp(-z) = inf gives 0
-  return __frcp_rn(1.0f + __expf(-z));
+  float r;  // 2^-22; exp(-z) = inf gives 0
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + __expf(-z)));
+  return r;
 }
 
 __device__ __forceinline__ float gated(float y, float z, int act) {
@@ -48,7 +51,17 @@ __device__ __forceinline__ float row_sum(float v, int lanes, float (*red)[32], i
   return v;
 }
 
-template <typename T, typename P, int V, int NV, bool CTA_ROW>
+// What a thread holds of a row as it was loaded.
+template <typename T, int V, int NV, bool GATE>
+struct Held {
+  Vec<T, V> x[NV], r[NV], g[GATE ? NV : 1];
+};
+
+// SHIFT: rows do not start on 16 bytes, but every tensor's row is as far past
+// a boundary as the others': vector c of a row is the aligned one that holds
+// its elements c V - off .. c V - off + V - 1, the first and the last of them
+// moved element by element.
+template <typename T, typename P, int V, int NV, bool CTA_ROW, bool GATE, bool SHIFT>
 __global__ void __launch_bounds__(CTA_ROW ? kMaxThreads : 128)
 block_norm_kernel(const __grid_constant__ exl3_block_norm_args a, int lanes) {
   __shared__ float red[2][32];
@@ -57,42 +70,80 @@ block_norm_kernel(const __grid_constant__ exl3_block_norm_args a, int lanes) {
   const int lane = CTA_ROW ? threadIdx.x : threadIdx.x & (lanes - 1);
   const int width = CTA_ROW ? blockDim.x : lanes;
   const int sub = CTA_ROW ? 0 : threadIdx.x / lanes;
-  const int nvec = (int)((a.d + V - 1) / V);
-  const float inv_d = 1.0f / (float)a.d;
+  const int d = (int)a.d;
+  const float inv_d = 1.0f / (float)d;
   using Vt = Vec<T, V>;
   using Vp = Vec<P, V>;
-  const T* x = static_cast<const T*>(a.x);
-  const T* gate = static_cast<const T*>(a.gate);
-  const T* residual = static_cast<const T*>(a.residual);
-  const P* weight = static_cast<const P*>(a.weight);
-  const P* next_weight = static_cast<const P*>(a.next_weight);
-  const P* scale = static_cast<const P*>(a.scale);
-  T* hidden = static_cast<T*>(a.hidden);
-  T* normed = static_cast<T*>(a.normed);
+  const T* const x = static_cast<const T*>(a.x);
+  const T* const gate = static_cast<const T*>(a.gate);
+  const T* const residual = static_cast<const T*>(a.residual);
+  const P* const weight = static_cast<const P*>(a.weight);
+  const P* const next_weight = static_cast<const P*>(a.next_weight);
+  const P* const scale = static_cast<const P*>(a.scale);
+  T* const hidden = static_cast<T*>(a.hidden);
+  T* const normed = static_cast<T*>(a.normed);
 
-  for (int64_t r0 = (int64_t)blockIdx.x * per_cta; r0 < a.rows; r0 += (int64_t)gridDim.x * per_cta) {
+  const auto offset = [&](int64_t row) {
+    return SHIFT ? (int)(reinterpret_cast<uintptr_t>(x + row * a.x_stride) / sizeof(T) % V) : 0;
+  };
+  // vector c of a row that starts at p: elements e0 .. e0 + V - 1
+  const auto load = [&](const T* p, int e0) {
+    if (!SHIFT || (e0 >= 0 && e0 + V <= d)) return *reinterpret_cast<const Vt*>(p + e0);
+    Vt v = {};
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (e0 + e >= 0 && e0 + e < d) v.e[e] = p[e0 + e];
+    return v;
+  };
+  const auto store = [&](T* p, int e0, const Vt& v) {
+    if (!SHIFT || (e0 >= 0 && e0 + V <= d)) {
+      *reinterpret_cast<Vt*>(p + e0) = v;
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (e0 + e >= 0 && e0 + e < d) p[e0 + e] = v.e[e];
+  };
+  const auto param = [&](const P* p, int e0) {
+    if (!SHIFT) return *reinterpret_cast<const Vp*>(p + e0);
+    Vp v;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const int at = e0 + e < 0 ? 0 : e0 + e < d ? e0 + e : d - 1;
+      v.e[e] = p[at];
+    }
+    return v;
+  };
+  const auto fetch = [&](int64_t row, Held<T, V, NV, GATE>& raw) {
+    const int off = offset(row);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e0 = (lane + i * width) * V - off;
+      raw.x[i] = {};
+      raw.r[i] = {};
+      if (GATE) raw.g[i] = {};
+      if (row < a.rows && e0 < d) {
+        raw.x[i] = load(x + row * a.x_stride, e0);
+        if (GATE) raw.g[i] = load(gate + row * a.gate_stride, e0);
+        if (residual) raw.r[i] = load(residual + row * a.residual_stride, e0);
+      }
+    }
+  };
+
+  const int64_t step = (int64_t)gridDim.x * per_cta;
+  Held<T, V, NV, GATE> ahead;
+  fetch((int64_t)blockIdx.x * per_cta + sub, ahead);
+  for (int64_t r0 = (int64_t)blockIdx.x * per_cta; r0 < a.rows; r0 += step) {
     // every thread of the warp takes part in the sums; rows past the end
     // compute on zeros and store nothing
     const int64_t row = r0 + sub;
     const bool live = row < a.rows;
+    const int off = offset(row);
+    const Held<T, V, NV, GATE> raw = ahead;
+    if (r0 + step < a.rows) fetch(row + step, ahead);
     float y[NV][V];
-    Vt gv[NV], rv[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = lane + i * width;
-      const bool in = live && c < nvec;
-      Vt xv = {};
-      gv[i] = {};
-      rv[i] = {};
-      if (in) {
-        xv = *reinterpret_cast<const Vt*>(x + row * a.x_stride + (int64_t)c * V);
-        if (gate) gv[i] = *reinterpret_cast<const Vt*>(gate + row * a.gate_stride + (int64_t)c * V);
-        if (residual)
-          rv[i] = *reinterpret_cast<const Vt*>(residual + row * a.residual_stride + (int64_t)c * V);
-      }
-#pragma unroll
-      for (int e = 0; e < V; ++e) y[i][e] = to_f32(xv.e[e]);
-    }
+    for (int i = 0; i < NV; ++i) unpack(raw.x[i], y[i]);
     if (weight) {
       float ss = 0.f;
 #pragma unroll
@@ -103,48 +154,49 @@ block_norm_kernel(const __grid_constant__ exl3_block_norm_args a, int lanes) {
       const float r = rsqrtf(ss * inv_d + a.eps);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = lane + i * width;
-        if (c >= nvec) break;
-        const Vp wv = *reinterpret_cast<const Vp*>(weight + (int64_t)c * V);
+        const int e0 = (lane + i * width) * V - off;
+        if (e0 >= d) break;
+        float w[V];
+        unpack(param(weight, e0), w);
 #pragma unroll
-        for (int e = 0; e < V; ++e) y[i][e] = y[i][e] * r * (a.weight_offset + to_f32(wv.e[e]));
+        for (int e = 0; e < V; ++e) y[i][e] = y[i][e] * r * (a.weight_offset + w[e]);
       }
     }
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = lane + i * width;
-      if (c >= nvec) break;
-      Vp sv = {};
-      if (scale) sv = *reinterpret_cast<const Vp*>(scale + (int64_t)c * V);
-      Vt hv;
+      const int e0 = (lane + i * width) * V - off;
+      if (e0 >= d) break;
+      float g[V], res[V], w[V];
+      if (GATE) unpack(raw.g[i], g);
+      unpack(raw.r[i], res);
+      if (scale) unpack(param(scale, e0), w);
+      float h[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        float h = y[i][e];
-        if (gate) h = gated(h, to_f32(gv[i].e[e]), a.gate_activation);
-        if (residual)
-          h = fmaf(scale ? a.residual_scale * to_f32(sv.e[e]) : a.residual_scale, h,
-                   to_f32(rv[i].e[e]));
-        y[i][e] = h;
-        ss = fmaf(h, h, ss);
-        hv.e[e] = from_f32<T>(h);
+        h[e] = y[i][e];
+        if (GATE) h[e] = gated(h[e], g[e], a.gate_activation);
+        if (residual) h[e] = fmaf(scale ? a.residual_scale * w[e] : a.residual_scale, h[e], res[e]);
+        // elements outside the row were loaded as zeros, but a zero gate's or
+        // sum's exact zero is not relied on
+        y[i][e] = SHIFT && (e0 + e < 0 || e0 + e >= d) ? 0.f : h[e];
+        ss = fmaf(y[i][e], y[i][e], ss);
       }
-      if (hidden && live)
-        *reinterpret_cast<Vt*>(hidden + row * a.hidden_stride + (int64_t)c * V) = hv;
+      const Vt hv = pack<T>(h);
+      if (hidden && live) store(hidden + row * a.hidden_stride, e0, hv);
     }
     if (next_weight) {
       ss = row_sum<CTA_ROW>(ss, lanes, red, slot);
       const float r = rsqrtf(ss * inv_d + a.eps);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = lane + i * width;
-        if (c >= nvec) break;
-        const Vp wv = *reinterpret_cast<const Vp*>(next_weight + (int64_t)c * V);
-        Vt nv;
+        const int e0 = (lane + i * width) * V - off;
+        if (e0 >= d) break;
+        float w[V];
+        unpack(param(next_weight, e0), w);
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          nv.e[e] = from_f32<T>(y[i][e] * r * (a.weight_offset + to_f32(wv.e[e])));
-        if (live) *reinterpret_cast<Vt*>(normed + row * a.normed_stride + (int64_t)c * V) = nv;
+        for (int e = 0; e < V; ++e) w[e] = y[i][e] * r * (a.weight_offset + w[e]);
+        if (live) store(normed + row * a.normed_stride, e0, pack<T>(w));
       }
     }
   }
@@ -202,52 +254,73 @@ block_norm_long_kernel(const __grid_constant__ exl3_block_norm_args a) {
   }
 }
 
-template <typename T, typename P, int V, int NV, bool CTA_ROW>
+template <typename T, typename P, int V, int NV, bool CTA_ROW, bool GATE, bool SHIFT>
 int launch(const exl3_block_norm_args& a, int threads, int lanes, cudaStream_t stream) {
+  const auto kernel = block_norm_kernel<T, P, V, NV, CTA_ROW, GATE, SHIFT>;
   const int per_cta = CTA_ROW ? 1 : threads / lanes;
   const int64_t ctas = (a.rows + per_cta - 1) / per_cta;
-  const int64_t most = (int64_t)sm_count() * 64;
-  block_norm_kernel<T, P, V, NV, CTA_ROW>
-      <<<(unsigned)(ctas < most ? ctas : most), threads, 0, stream>>>(a, lanes);
+  // as many CTAs as run at once: each has a next row to load
+  static std::atomic<int> known[kMaxThreads / 32 + 1];  // by warps of a CTA
+  int resident = known[threads / 32].load(std::memory_order_relaxed);
+  if (resident == 0) {
+    EXL3_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, threads, 0));
+    if (resident < 1) resident = 1;
+    known[threads / 32].store(resident, std::memory_order_relaxed);
+  }
+  const int64_t most = (int64_t)sm_count() * resident;
+  kernel<<<(unsigned)(ctas < most ? ctas : most), threads, 0, stream>>>(a, lanes);
   EXL3_LAUNCHED();
   return EXL3_OK;
 }
 
-template <typename T, typename P, int V>
+template <typename T, typename P, int V, bool GATE, bool SHIFT>
 int launch_v(const exl3_block_norm_args& a, cudaStream_t stream) {
-  const int64_t nvec = (a.d + V - 1) / V;
+  // a shifted row may reach into one vector more
+  const int64_t nvec = (a.d + V - 1) / V + (SHIFT ? 1 : 0);
   if (nvec <= 128) {
     int lanes = 1;
     while (lanes < nvec && lanes < 32) lanes *= 2;
-    if (nvec <= lanes) return launch<T, P, V, 1, false>(a, 128, lanes, stream);
-    if (nvec <= 2 * lanes) return launch<T, P, V, 2, false>(a, 128, lanes, stream);
-    return launch<T, P, V, 4, false>(a, 128, lanes, stream);
+    if (nvec <= lanes) return launch<T, P, V, 1, false, GATE, SHIFT>(a, 128, lanes, stream);
+    if (nvec <= 2 * lanes) return launch<T, P, V, 2, false, GATE, SHIFT>(a, 128, lanes, stream);
+    return launch<T, P, V, 4, false, GATE, SHIFT>(a, 128, lanes, stream);
   }
   const auto threads = [&](int nv) { return (int)((nvec + 32 * nv - 1) / (32 * nv)) * 32; };
   // few rows: as many threads as there are vectors; else two vectors each
   if (nvec <= kMaxThreads && a.rows <= sm_count())
-    return launch<T, P, V, 1, true>(a, threads(1), 32, stream);
-  if (nvec <= 2 * kMaxThreads) return launch<T, P, V, 2, true>(a, threads(2), 32, stream);
-  if (nvec <= 4 * kMaxThreads) return launch<T, P, V, 4, true>(a, threads(4), 32, stream);
-  const int64_t most = (int64_t)sm_count() * 16;
+    return launch<T, P, V, 1, true, GATE, SHIFT>(a, threads(1), 32, stream);
+  if (nvec <= 2 * kMaxThreads) return launch<T, P, V, 2, true, GATE, SHIFT>(a, threads(2), 32, stream);
+  if (nvec <= 4 * kMaxThreads) return launch<T, P, V, 4, true, GATE, SHIFT>(a, threads(4), 32, stream);
+  const int64_t most = (int64_t)sm_count() * 2;
   block_norm_long_kernel<T, P>
       <<<(unsigned)(a.rows < most ? a.rows : most), 1024, 0, stream>>>(a);
   EXL3_LAUNCHED();
   return EXL3_OK;
 }
 
+template <typename T, typename P, int V, bool SHIFT>
+int launch_g(const exl3_block_norm_args& a, cudaStream_t stream) {
+  return a.gate ? launch_v<T, P, V, true, SHIFT>(a, stream) : launch_v<T, P, V, false, SHIFT>(a, stream);
+}
+
 template <typename T, typename P>
 int launch_t(const exl3_block_norm_args& a, cudaStream_t stream) {
   constexpr int V = 16 / sizeof(T);
-  const auto row_ok = [](const void* p, int64_t stride) {
-    return !p || (aligned_to(p, 16) && stride % V == 0);
-  };
-  const auto vec_ok = [](const void* p) { return !p || aligned_to(p, V * sizeof(P)); };
-  const bool wide = a.d % V == 0 && row_ok(a.x, a.x_stride) && row_ok(a.gate, a.gate_stride) &&
-                    row_ok(a.residual, a.residual_stride) && row_ok(a.hidden, a.hidden_stride) &&
-                    row_ok(a.normed, a.normed_stride) && vec_ok(a.weight) &&
-                    vec_ok(a.next_weight) && vec_ok(a.scale);
-  return wide ? launch_v<T, P, V>(a, stream) : launch_v<T, P, 1>(a, stream);
+  const struct { const void* p; int64_t stride; } rows[] = {
+      {a.x, a.x_stride}, {a.gate, a.gate_stride}, {a.residual, a.residual_stride},
+      {a.hidden, a.hidden_stride}, {a.normed, a.normed_stride}};
+  bool wide = a.d % V == 0, alike = true;
+  for (const auto& r : rows) {
+    if (!r.p) continue;
+    wide = wide && aligned_to(r.p, 16) && r.stride % V == 0;
+    alike = alike && reinterpret_cast<uintptr_t>(r.p) % sizeof(T) == 0 &&
+            (reinterpret_cast<uintptr_t>(r.p) - reinterpret_cast<uintptr_t>(a.x)) % 16 == 0 &&
+            (r.stride - a.x_stride) % V == 0;
+  }
+  for (const void* p : {a.weight, a.next_weight, a.scale}) wide = wide && (!p || aligned_to(p, V * sizeof(P)));
+  // vectors, vectors from each row's boundary on, or element by element
+  if (wide) return launch_g<T, P, V, false>(a, stream);
+  if (alike && a.d >= 4 * V) return launch_g<T, P, V, true>(a, stream);
+  return launch_g<T, P, 1, false>(a, stream);
 }
 
 }  // namespace

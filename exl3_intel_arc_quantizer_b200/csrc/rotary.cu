@@ -39,12 +39,21 @@ __device__ __forceinline__ uint64_t turn_step(float inv_freq) {
   return __double2ull_rz(head * 0x1p64) + __double2ull_rz(tail * 0x1p64);
 }
 
+// Place of pair j in a token's row of the table: a thread reads V pairs, 16
+// bytes (two pairs) at a time, and V = 8 puts the threads 64 bytes apart; the
+// 16-byte pieces of a thread's 64 are permuted so that 8 threads use all banks
+// twice instead of half of them four times.
+template <int V>
+__device__ __forceinline__ int table_at(int j) {
+  return V == 8 ? (j & ~7) | ((j & 7) ^ ((j >> 2) & 6)) : j;
+}
+
 // An item is what a thread turns at once: V pairs (two vectors of the half
 // layout, or 2V neighbouring elements = two vectors, interleaved), or two
 // vectors of the part that is copied.
 template <typename T, int V, bool INTER>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryLaunch p) {
-  extern __shared__ float2 cs[];  // [tokens][rotary_dim / 2]: factor * (cos, sin)
+  extern __shared__ __align__(16) float2 cs[];  // [tokens][rotary_dim / 2]: factor * (cos, sin)
   const exl3_rotary_args& a = p.a;
   const int half = a.rotary_dim / 2, tid = threadIdx.x;
   const int64_t blocks = (a.tokens + p.tokens_per_cta - 1) / p.tokens_per_cta;
@@ -53,20 +62,10 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
   const int h0 = blockIdx.y * p.heads_per_cta;
   const int heads = a.q_heads + a.k_heads;
   const int nh = heads - h0 < p.heads_per_cta ? heads - h0 : p.heads_per_cta;
-
-  for (int i = tid; i < nt * half; i += kThreads) {
-    const int t = i / half, j = i - t * half;
-    const int64_t at = b * a.position_strides[0] + (t0 + t) * a.position_strides[1];
-    const int64_t pos = a.positions_64 ? static_cast<const int64_t*>(a.positions)[at]
-                                       : static_cast<const int32_t*>(a.positions)[at];
-    const uint64_t step = turn_step(a.inv_freq[j]);
-    const int64_t phase = (int64_t)((uint64_t)pos * step);
-    float s, c;
-    sincospif(__ll2float_rn(phase) * 1.0842021724855044e-19f, &s, &c);  // 2^-63: half turns
-    if (a.transposed) s = -s;
-    cs[i] = make_float2(a.factor * c, a.factor * s);
-  }
-  __syncthreads();
+  const T* const q = static_cast<const T*>(a.q) + b * a.q_strides[0] + t0 * a.q_strides[1];
+  const T* const k = static_cast<const T*>(a.k) + b * a.k_strides[0] + t0 * a.k_strides[1];
+  T* const qo = static_cast<T*>(a.q_out) + b * a.q_out_strides[0] + t0 * a.q_out_strides[1];
+  T* const ko = static_cast<T*>(a.k_out) + b * a.k_out_strides[0] + t0 * a.k_out_strides[1];
 
   const int turned = half / V;                                   // items that turn, per head
   const int copied = (a.dim - a.rotary_dim) / V;                 // vectors that are copied
@@ -74,56 +73,78 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
   const int lane = tid & (p.lanes - 1), groups = kThreads / p.lanes;
   const int pairs = nt * nh;
   using Ve = Vec<T, V>;
-  for (int i0 = lane; i0 < items; i0 += p.lanes) {
+  bool table = false;
+  const int first = tid / p.lanes, first_t = first / nh;
+  for (int i0 = lane; i0 < items || !table; i0 += p.lanes) {
     const bool turn = i0 < turned;
     const int e0 = turn ? (INTER ? 2 * V * i0 : V * i0) : a.rotary_dim + 2 * V * (i0 - turned);
     const int e1 = turn ? (INTER ? e0 + V : e0 + half) : e0 + V;
-    const bool second = e1 < a.dim;
-    for (int p0 = tid / p.lanes; p0 < pairs; p0 += groups * kUnroll) {
+    const bool second = e1 < a.dim, live = i0 < items;
+    int t = first_t, h = first - first_t * nh;
+    for (int p0 = first; p0 < pairs || !table; p0 += groups * kUnroll) {
       Ve x0[kUnroll], x1[kUnroll];
       T* dst[kUnroll];
-      const float2* tab[kUnroll];
+      int row[kUnroll];
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
-        const int pr = p0 + u * groups;
-        if (pr >= pairs) break;
-        const int t = pr / nh, h = h0 + pr - t * nh;
-        const bool isq = h < a.q_heads;
-        const int hh = isq ? h : h - a.q_heads;
-        const int64_t* si = isq ? a.q_strides : a.k_strides;
-        const int64_t* so = isq ? a.q_out_strides : a.k_out_strides;
-        const T* src = static_cast<const T*>(isq ? a.q : a.k) + b * si[0] + (t0 + t) * si[1] + hh * si[2];
-        dst[u] = static_cast<T*>(isq ? a.q_out : a.k_out) + b * so[0] + (t0 + t) * so[1] + hh * so[2];
-        tab[u] = cs + t * half + V * i0;
-        x0[u] = *reinterpret_cast<const Ve*>(src + e0);
-        if (second) x1[u] = *reinterpret_cast<const Ve*>(src + e1);
+        if (live && p0 + u * groups < pairs) {
+          const int hh = h0 + h - a.q_heads;
+          const T* src = hh < 0 ? q + t * a.q_strides[1] + (h0 + h) * a.q_strides[2]
+                                : k + t * a.k_strides[1] + hh * a.k_strides[2];
+          dst[u] = hh < 0 ? qo + t * a.q_out_strides[1] + (h0 + h) * a.q_out_strides[2]
+                          : ko + t * a.k_out_strides[1] + hh * a.k_out_strides[2];
+          row[u] = t * half;
+          x0[u] = *reinterpret_cast<const Ve*>(src + e0);
+          if (second) x1[u] = *reinterpret_cast<const Ve*>(src + e1);
+        }
+        for (h += groups; h >= nh; h -= nh) ++t;
+      }
+      // the table is made while the first vectors are on their way
+      if (!table) {
+        for (int i = tid; i < nt * half; i += kThreads) {
+          const int tt = i / half, j = i - tt * half;
+          const int64_t at = b * a.position_strides[0] + (t0 + tt) * a.position_strides[1];
+          const int64_t pos = a.positions_64 ? static_cast<const int64_t*>(a.positions)[at]
+                                             : static_cast<const int32_t*>(a.positions)[at];
+          const int64_t phase = (int64_t)((uint64_t)pos * turn_step(a.inv_freq[j]));
+          float s, c;
+          sincospif(__ll2float_rn(phase) * 1.0842021724855044e-19f, &s, &c);  // 2^-63: half turns
+          if (a.transposed) s = -s;
+          cs[tt * half + table_at<V>(j)] = make_float2(a.factor * c, a.factor * s);
+        }
+        __syncthreads();
+        table = true;
       }
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
-        if (p0 + u * groups >= pairs) break;
+        if (!live || p0 + u * groups >= pairs) break;
         if (turn) {
-          if constexpr (INTER) {
-            T* y0 = x0[u].e;
-            T* y1 = x1[u].e;
+          float2 w[V];
 #pragma unroll
-            for (int m = 0; m < V; ++m) {
-              // pair m holds elements 2m and 2m + 1 of the two vectors
-              T& ea = (2 * m < V) ? y0[(2 * m) % V] : y1[(2 * m) % V];
-              T& eb = (2 * m + 1 < V) ? y0[(2 * m + 1) % V] : y1[(2 * m + 1) % V];
-              const float2 w = tab[u][m];
-              const float va = to_f32(ea), vb = to_f32(eb);
-              ea = from_f32<T>(va * w.x - vb * w.y);
-              eb = from_f32<T>(vb * w.x + va * w.y);
-            }
-          } else {
-#pragma unroll
-            for (int m = 0; m < V; ++m) {
-              const float2 w = tab[u][m];
-              const float va = to_f32(x0[u].e[m]), vb = to_f32(x1[u].e[m]);
-              x0[u].e[m] = from_f32<T>(va * w.x - vb * w.y);
-              x1[u].e[m] = from_f32<T>(vb * w.x + va * w.y);
+          for (int m = 0; m < V; m += V > 1 ? 2 : 1) {
+            const float2* at = cs + row[u] + table_at<V>(V * i0 + m);
+            if constexpr (V > 1) {
+              const float4 two = *reinterpret_cast<const float4*>(at);
+              w[m] = make_float2(two.x, two.y);
+              w[m + 1] = make_float2(two.z, two.w);
+            } else {
+              w[m] = *at;
             }
           }
+          float f0[V], f1[V];
+          unpack(x0[u], f0);
+          unpack(x1[u], f1);
+#pragma unroll
+          for (int m = 0; m < V; ++m) {
+            // interleaved: pair m holds elements 2m and 2m + 1 of the two vectors
+            float& ea = INTER ? (2 * m < V ? f0[(2 * m) % V] : f1[(2 * m) % V]) : f0[m];
+            float& eb = INTER ? (2 * m + 1 < V ? f0[(2 * m + 1) % V] : f1[(2 * m + 1) % V]) : f1[m];
+            const float va = ea, vb = eb;
+            ea = va * w[m].x - vb * w[m].y;
+            eb = vb * w[m].x + va * w[m].y;
+          }
+          x0[u] = pack<T>(f0);
+          x1[u] = pack<T>(f1);
         }
         *reinterpret_cast<Ve*>(dst[u] + e0) = x0[u];
         if (second) *reinterpret_cast<Ve*>(dst[u] + e1) = x1[u];
@@ -141,14 +162,14 @@ int launch(const exl3_rotary_args& a, cudaStream_t stream) {
   p.lanes = 1;
   while (p.lanes < items && p.lanes < 32) p.lanes *= 2;
   // few tokens: a CTA takes one token and as many heads as its threads hold
-  // at once; many tokens: all heads, and tokens for four rounds of loads
+  // at once; many tokens: all heads, and tokens for one round of loads
   const int groups = kThreads / p.lanes;
-  int tokens = 1;
-  while (tokens * heads < groups * kUnroll && tokens * 2 * half * 8 <= 32768 &&
-         a.batch * ((a.tokens + 2 * tokens - 1) / (2 * tokens)) >= 4 * sm_count())
-    tokens *= 2;
+  const bool many = a.batch * a.tokens >= 4 * sm_count();
+  int tokens = many ? groups * kUnroll / heads : 1;
+  const int fit = 32768 / (half * (int)sizeof(float2));
+  tokens = tokens < 1 ? 1 : tokens > fit ? fit : tokens;
   p.tokens_per_cta = tokens;
-  p.heads_per_cta = a.batch * a.tokens >= 4 * sm_count() ? heads : (groups < heads ? groups : heads);
+  p.heads_per_cta = many || groups >= heads ? heads : groups;
   const int64_t bx = a.batch * ((a.tokens + tokens - 1) / tokens);
   const int by = (heads + p.heads_per_cta - 1) / p.heads_per_cta;
   EXL3_REQUIRE(bx < (1ll << 31) && by < 65536, "too many tokens or heads");
