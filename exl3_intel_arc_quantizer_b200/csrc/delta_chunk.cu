@@ -46,6 +46,7 @@
 
 #include "common.cuh"
 #include "delta_rule.cuh"
+#include "pipeline.cuh"
 
 namespace exl3 {
 
@@ -69,10 +70,6 @@ constexpr int64_t kHeadBytes = kImageBytes + kVecFloats * 4;
 __device__ __forceinline__ int64_t slot_base(int64_t t0, int64_t s) { return t0 / kChunk + s; }
 __host__ __device__ __forceinline__ int64_t slot_bytes(const exl3_delta_args& a) {
   return (int64_t)a.key_heads * kKqBytes + (int64_t)a.heads * kHeadBytes;
-}
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
 // Byte of 16-byte piece q of row r in a 128-byte-swizzled operand tile
@@ -109,10 +106,10 @@ __device__ __forceinline__ void pow2_scale(float bound, float& scale, float& inv
 template <typename T>
 __device__ __forceinline__ uint4 load8(const T* p, bool vec) {
   if (vec) return *reinterpret_cast<const uint4*>(p);
-  Vec<T, 8> v;
+  uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v.e[i] = p[i];
-  return *reinterpret_cast<const uint4*>(&v);
+  for (int i = 0; i < 4; ++i) w[i] = f32_to_word<T>(make_float2(to_f32(p[2 * i]), to_f32(p[2 * i + 1])));
+  return make_uint4(w[0], w[1], w[2], w[3]);  // the elements' own values again
 }
 
 // ---------------------------------------------------------------------------
@@ -222,10 +219,8 @@ delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int r = (tid >> 4) + 16 * i;
-      const T* e = reinterpret_cast<const T*>(&x[i]);
       float f[8], ss = 0.f, back = 1.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = to_f32(e[j]);
+      unpack(Raw<T, 8>{{x[i].x, x[i].y, x[i].z, x[i].w}}, f);
       if constexpr (!std::is_same<T, __half>::value) {
         // the row's largest element goes to [1, 2)
         float big = 0.f;
@@ -630,8 +625,6 @@ delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict
 // The chain of states
 // ---------------------------------------------------------------------------
 
-constexpr long long kWaitClocks = 4000000000ll;  // 2 s per wait at 2 GHz
-
 // GROUPS column groups of NV columns, each with its own barriers, tensor
 // memory and issuing warp (one group's products run under the other's
 // elementwise steps); CT columns per epilogue thread. The high and low parts
@@ -662,47 +655,6 @@ struct Geo {
   static_assert(kTBytes % 1024 == 0 && kOpBytes % 1024 == 0, "operand tiles start on 1,024 bytes");
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
-
-__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
-}
-__device__ __forceinline__ void bar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.b32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// true when the phase completed; false on timeout (which raises the abort
-// flag) or when another role has aborted
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  long long start = 0;
-  for (uint32_t it = 1;; ++it) {
-    if (bar_try(bar, parity)) return true;
-    if ((it & 63u) == 0u) {
-      if (*abort_flag) return false;
-      const long long now = clock64();
-      if (start == 0) start = now;
-      if (now - start > kWaitClocks) {
-        *abort_flag = 1;
-        return false;
-      }
-    }
-  }
-}
-// the shutdown path's wait: bounded, whatever the abort flag says
-__device__ __forceinline__ void bar_drain(uint32_t bar, uint32_t parity) {
-  const long long start = clock64();
-  while (!bar_try(bar, parity))
-    if (clock64() - start > kWaitClocks) return;
-}
 
 // Operand descriptor of a 128-byte-swizzled tile (8-row groups 1,024 bytes
 // apart): this is the low word, the high one is kDescHigh. lbo is the distance
@@ -845,7 +797,7 @@ delta_chain_kernel(const __grid_constant__ exl3_delta_args a, const uint8_t* __r
     }
     *abort_flag = 0;
     for (int i = 0; i < 4 * GROUPS; ++i) (&peak[0][0][0])[i] = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    bar_init_fence();
   }
   if (warp == L::kEpiWarps) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -989,14 +941,13 @@ delta_chain_kernel(const __grid_constant__ exl3_delta_args a, const uint8_t* __r
         for (int c = 0; c < CT; c += 8) {
           load2(d1, c, f, l);
           const uint4 x = load_v(ch, c / 8);
-          const T* ve = reinterpret_cast<const T*>(&x);
+          const uint32_t ve[4] = {x.x, x.y, x.z, x.w};
           tmem_ld_wait();
           add2(f, l);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             f[i] = __ffma2_rn(make_float2(m, m), f[i],
-                              __fmul2_rn(make_float2(to_f32(ve[2 * i]), to_f32(ve[2 * i + 1])),
-                                         make_float2(scale_r, scale_r)));
+                              __fmul2_rn(word_to_f32<T>(ve[i]), make_float2(scale_r, scale_r)));
           store_op(64 * 128, c, f, peak2);
         }
         ready(1);
@@ -1038,16 +989,14 @@ delta_chain_kernel(const __grid_constant__ exl3_delta_args a, const uint8_t* __r
           }
           add2(f, l);
           add2(p, pl);
-          Vec<T, 8> y;
+          uint32_t y[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float2 x = __ffma2_rn(make_float2(ab, ab), f[i],
-                                        __fmul2_rn(make_float2(from_image, from_image), p[i]));
-            y.e[2 * i] = from_f32<T>(x.x);
-            y.e[2 * i + 1] = from_f32<T>(x.y);
+            y[i] = f32_to_word<T>(__ffma2_rn(make_float2(ab, ab), f[i],
+                                             __fmul2_rn(make_float2(from_image, from_image), p[i])));
           }
           if (t < t1 && col + c < a.dv)
-            *reinterpret_cast<uint4*>(o + c) = *reinterpret_cast<const uint4*>(&y);
+            *reinterpret_cast<uint4*>(o + c) = make_uint4(y[0], y[1], y[2], y[3]);
         }
       }
       // 3. the state moves on
@@ -1151,17 +1100,6 @@ delta_chain_kernel(const __grid_constant__ exl3_delta_args a, const uint8_t* __r
     bar_drain(gbar(g, 6), 0);
   } else {
     // ---------------- copies ----------------
-    const auto expect = [&](uint32_t full, uint32_t bytes) {
-      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full), "r"(bytes)
-                   : "memory");
-    };
-    const auto copy = [&](uint8_t* dst, const void* src, uint32_t bytes, uint32_t full) {
-      asm volatile(
-          "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-              smem_u32(dst)),
-          "l"(src), "r"(bytes), "r"(full)
-          : "memory");
-    };
     const T* v = static_cast<const T*>(a.v) + h * a.v_strides[1] + col_base;
     const int v_cols = col_end - col_base;
     int kq_issued = 0, t_issued = 0;
@@ -1171,8 +1109,8 @@ delta_chain_kernel(const __grid_constant__ exl3_delta_args a, const uint8_t* __r
       if (ch >= L::kKQStages) ok = bar_wait(kq_empty(ks), (ch / L::kKQStages - 1) & 1, abort_flag);
       if (!__all_sync(0xFFFFFFFFu, ok)) break;
       if (lane == 0) {
-        expect(kq_full(ks), kKqBytes);
-        copy(kq_base + ks * kKqBytes, kq_img + ch * img_step, kKqBytes, kq_full(ks));
+        bar_expect(kq_full(ks), kKqBytes);
+        bulk_load(kq_base + ks * kKqBytes, kq_img + ch * img_step, kKqBytes, kq_full(ks));
       }
       kq_issued = ch + 1;
       if (ch >= L::kTStages) ok = bar_wait(t_empty(ts), (ch / L::kTStages - 1) & 1, abort_flag);
@@ -1181,8 +1119,8 @@ delta_chain_kernel(const __grid_constant__ exl3_delta_args a, const uint8_t* __r
       const int64_t tc = t0 + (int64_t)ch * kChunk;
       const int n = (int)(t1 - tc < kChunk ? t1 - tc : kChunk);
       if (lane == 0) {
-        expect(t_full(ts), kHeadBytes);
-        copy(tile, img + ch * img_step, kHeadBytes, t_full(ts));
+        bar_expect(t_full(ts), kHeadBytes);
+        bulk_load(tile, img + ch * img_step, kHeadBytes, t_full(ts));
       }
       // v in 16-byte pieces; zeros for rows past the sequence, whatever
       // follows it in memory, and for columns past dv
@@ -1278,9 +1216,12 @@ int delta_chunks(const exl3_delta_args& a, void* ws, cudaStream_t stream) {
 
 }  // namespace exl3
 
-extern "C" int exl3_delta_fault_count(unsigned int* count) {
+extern "C" int exl3_layer_fault_count(unsigned int* count) {
   using namespace exl3;
   EXL3_REQUIRE(count != nullptr, "count is NULL");
-  EXL3_CUDA(cudaMemcpyFromSymbol(count, g_delta_faults, sizeof(unsigned int)));
+  unsigned int delta = 0, norm = 0;
+  EXL3_CUDA(cudaMemcpyFromSymbol(&delta, g_delta_faults, sizeof(unsigned int)));
+  if (const int rc = norm_fault_count(&norm)) return rc;
+  *count = delta + norm;
   return EXL3_OK;
 }

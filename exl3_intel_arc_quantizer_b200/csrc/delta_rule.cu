@@ -29,9 +29,10 @@ __device__ __forceinline__ void load_row(const T* p, int at, int d, bool vec, fl
 #pragma unroll
     for (int c = 0; c < N; c += 8) {
       if (at + c < d) {  // d is a multiple of 8
-        const Vec<T, 8> v = *reinterpret_cast<const Vec<T, 8>*>(p + at + c);
+        float f[8];
+        unpack(load_raw<T, 8>(p + at + c), f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) out[c + i] = to_f32(v.e[i]);
+        for (int i = 0; i < 8; ++i) out[c + i] = f[i];
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) out[c + i] = 0.f;
@@ -121,12 +122,11 @@ delta_tokens_kernel(const __grid_constant__ exl3_delta_args a, int vec) {
       for (int j = 0; j < 11; ++j) r[j] += __shfl_xor_sync(0xFFFFFFFFu, r[j], o);
     const float rk = a.normalize_qk ? rsqrtf(r[0] + kNormEps) : 1.f;
     const float rq = (a.normalize_qk ? rsqrtf(r[1] + kNormEps) : 1.f) * a.scale;
-    float u[4];
-    Vec<T, 4> o;
+    float u[4], o[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       u[c] = beta * (vr[c] - G * rk * r[3 + c]);
-      o.e[c] = from_f32<T>(rq * (G * r[7 + c] + r[2] * rk * u[c]));
+      o[c] = rq * (G * r[7 + c] + r[2] * rk * u[c]);
     }
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
@@ -135,7 +135,8 @@ delta_tokens_kernel(const __grid_constant__ exl3_delta_args a, int vec) {
       for (int c = 0; c < 4; ++c) S[i][c] = fmaf(ki, u[c], G * S[i][c]);
     }
     if (in && lane < CL)
-      *reinterpret_cast<Vec<T, 4>*>(static_cast<T*>(a.out) + (t * a.heads + h) * a.dv + col) = o;
+      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (t * a.heads + h) * a.dv + col) =
+          make_uint2(f32_to_word<T>(make_float2(o[0], o[1])), f32_to_word<T>(make_float2(o[2], o[3])));
   }
   if (in)
 #pragma unroll

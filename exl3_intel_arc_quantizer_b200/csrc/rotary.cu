@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
   const int items = turned + (copied + 1) / 2;
   const int lane = tid & (p.lanes - 1), groups = kThreads / p.lanes;
   const int pairs = nt * nh;
-  using Ve = Vec<T, V>;
+  using Ve = typename Pieces<T, V>::type;
   bool table = false;
   const int first = tid / p.lanes, first_t = first / nh;
   for (int i0 = lane; i0 < items || !table; i0 += p.lanes) {
@@ -94,8 +94,8 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
           dst[u] = hh < 0 ? qo + t * a.q_out_strides[1] + (h0 + h) * a.q_out_strides[2]
                           : ko + t * a.k_out_strides[1] + hh * a.k_out_strides[2];
           row[u] = t * half;
-          x0[u] = *reinterpret_cast<const Ve*>(src + e0);
-          if (second) x1[u] = *reinterpret_cast<const Ve*>(src + e1);
+          x0[u] = load_piece<T, V>(src + e0);
+          if (second) x1[u] = load_piece<T, V>(src + e1);
         }
         for (h += groups; h >= nh; h -= nh) ++t;
       }
@@ -143,11 +143,15 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
             ea = va * w[m].x - vb * w[m].y;
             eb = vb * w[m].x + va * w[m].y;
           }
-          x0[u] = pack<T>(f0);
-          x1[u] = pack<T>(f1);
+          store_piece<T, V>(dst[u] + e0, f0);
+          store_piece<T, V>(dst[u] + e1, f1);
+        } else if constexpr (V > 1) {
+          store_raw<T, V>(dst[u] + e0, x0[u]);
+          if (second) store_raw<T, V>(dst[u] + e1, x1[u]);
+        } else {
+          dst[u][e0] = from_f32<T>(x0[u]);  // the element's own value again
+          if (second) dst[u][e1] = from_f32<T>(x1[u]);
         }
-        *reinterpret_cast<Ve*>(dst[u] + e0) = x0[u];
-        if (second) *reinterpret_cast<Ve*>(dst[u] + e1) = x1[u];
       }
     }
   }

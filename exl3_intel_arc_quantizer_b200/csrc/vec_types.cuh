@@ -23,64 +23,123 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) {
   return __float2bfloat16_rn(x);
 }
 
-// V elements loaded and stored at once (one 16-byte access where they fill it)
+// V elements as 32-bit words, the way they are loaded, selected and stored (a
+// struct of 16-bit elements makes the compiler move each element by itself)
 template <typename T, int V>
-struct alignas(sizeof(T) * V) Vec {
-  T e[V];
+struct Raw {
+  static constexpr int kWords = V * (int)sizeof(T) / 4;
+  static_assert(V * sizeof(T) % 4 == 0, "whole words");
+  uint32_t w[kWords];
 };
 
-// Two elements at a time: one conversion instruction per pair on the way back
-__device__ __forceinline__ float2 to_f32x2(const Vec<__half, 2>& v) {
-  return __half22float2(*reinterpret_cast<const __half2*>(&v));
-}
-__device__ __forceinline__ float2 to_f32x2(const Vec<__nv_bfloat16, 2>& v) {
-  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
-}
-__device__ __forceinline__ float2 to_f32x2(const Vec<float, 2>& v) {
-  return make_float2(v.e[0], v.e[1]);
-}
-template <typename T>
-__device__ __forceinline__ Vec<T, 2> from_f32x2(float2 f);
-template <>
-__device__ __forceinline__ Vec<__half, 2> from_f32x2<__half>(float2 f) {
-  const __half2 h = __float22half2_rn(f);
-  return *reinterpret_cast<const Vec<__half, 2>*>(&h);
-}
-template <>
-__device__ __forceinline__ Vec<__nv_bfloat16, 2> from_f32x2<__nv_bfloat16>(float2 f) {
-  const __nv_bfloat162 h = __float22bfloat162_rn(f);
-  return *reinterpret_cast<const Vec<__nv_bfloat16, 2>*>(&h);
-}
-template <>
-__device__ __forceinline__ Vec<float, 2> from_f32x2<float>(float2 f) {
-  return {{f.x, f.y}};
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> load_raw(const T* p) {
+  Raw<T, V> r;
+  constexpr int n = Raw<T, V>::kWords;
+  if constexpr (n % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < n; i += 4) {
+      const uint4 x = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i);
+      r.w[i] = x.x;
+      r.w[i + 1] = x.y;
+      r.w[i + 2] = x.z;
+      r.w[i + 3] = x.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < n; ++i) r.w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+  }
+  return r;
 }
 template <typename T, int V>
-__device__ __forceinline__ void unpack(const Vec<T, V>& v, float (&f)[V]) {
-  if constexpr (V == 1) {
-    f[0] = to_f32(v.e[0]);
+__device__ __forceinline__ void store_raw(T* p, const Raw<T, V>& r) {
+  constexpr int n = Raw<T, V>::kWords;
+  if constexpr (n % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < n; i += 4)
+      *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(p) + i) =
+          make_uint4(r.w[i], r.w[i + 1], r.w[i + 2], r.w[i + 3]);
   } else {
-    const Vec<T, 2>* p = reinterpret_cast<const Vec<T, 2>*>(&v);
+#pragma unroll
+    for (int i = 0; i < n; ++i) reinterpret_cast<uint32_t*>(p)[i] = r.w[i];
+  }
+}
+
+// a word of two 16-bit elements
+template <typename T>
+__device__ __forceinline__ float2 word_to_f32(uint32_t w);
+template <>
+__device__ __forceinline__ float2 word_to_f32<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <>
+__device__ __forceinline__ float2 word_to_f32<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t f32_to_word(float2 f);
+template <>
+__device__ __forceinline__ uint32_t f32_to_word<__half>(float2 f) {
+  const __half2 h = __float22half2_rn(f);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t f32_to_word<__nv_bfloat16>(float2 f) {
+  const __nv_bfloat162 h = __float22bfloat162_rn(f);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Raw<T, V>& r, float (&f)[V]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = __uint_as_float(r.w[i]);
+  } else {
 #pragma unroll
     for (int i = 0; i < V / 2; ++i) {
-      const float2 x = to_f32x2(p[i]);
+      const float2 x = word_to_f32<T>(r.w[i]);
       f[2 * i] = x.x;
       f[2 * i + 1] = x.y;
     }
   }
 }
 template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> pack(const float (&f)[V]) {
-  Vec<T, V> v;
-  if constexpr (V == 1) {
-    v.e[0] = from_f32<T>(f[0]);
-  } else {
-    Vec<T, 2>* p = reinterpret_cast<Vec<T, 2>*>(&v);
+__device__ __forceinline__ Raw<T, V> pack(const float (&f)[V]) {
+  Raw<T, V> r;
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < V / 2; ++i) p[i] = from_f32x2<T>(make_float2(f[2 * i], f[2 * i + 1]));
+    for (int i = 0; i < V; ++i) r.w[i] = __float_as_uint(f[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) r.w[i] = f32_to_word<T>(make_float2(f[2 * i], f[2 * i + 1]));
   }
-  return v;
+  return r;
 }
+
+// The same for single elements, which have no words of their own
+template <typename T, int V>
+struct Pieces {
+  using type = Raw<T, V>;
+};
+template <typename T>
+struct Pieces<T, 1> {
+  using type = float;
+};
+template <typename T, int V>
+__device__ __forceinline__ typename Pieces<T, V>::type load_piece(const T* p) {
+  if constexpr (V == 1)
+    return to_f32(*p);
+  else
+    return load_raw<T, V>(p);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_piece(T* p, const float (&f)[V]) {
+  if constexpr (V == 1)
+    *p = from_f32<T>(f[0]);
+  else
+    store_raw<T, V>(p, pack<T, V>(f));
+}
+__device__ __forceinline__ void unpack(float x, float (&f)[1]) { f[0] = x; }
 
 inline bool aligned_to(const void* p, size_t bytes) {
   return reinterpret_cast<uintptr_t>(p) % bytes == 0;

@@ -174,3 +174,35 @@ def test_refusals():
         block_norm(x.double(), next_weight=w)
     with pytest.raises(RuntimeError, match="no_grad"):
         block_norm(x, next_weight=torch.nn.Parameter(w))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [8, 24, 64, 128, 136, 256, 264, 520, 1024, 2048, 4096, 8192])
+def test_many_rows(dtype, d):
+    """Enough rows for the tiles: whole ones, a last one that is not full."""
+    rows = 1501 if d <= 1024 else 701
+    run_and_check(*inputs(rows, d, dtype, dtype, "wgrn"))
+    run_and_check(*inputs(rows, d, dtype, torch.float32, "wGrsn"))
+    run_and_check(*inputs(rows, d, dtype, dtype, "n"))
+
+
+@pytest.mark.parametrize("d", [33, 63, 129, 250, 517, 1023, 2047, 4093, 4095])
+def test_many_odd_rows(d):
+    for dtype in (torch.float16, torch.float32):
+        run_and_check(*inputs(1203, d, dtype, dtype, "wgrn"))
+        run_and_check(*inputs(1203, d, dtype, torch.float32, "rsn"))
+    # all tensors equally far past a boundary, and not
+    for shifts in ((1, 1, 1), (3, 3, 3), (1, 2, 3)):
+        flat = [rand(700 * d + 8, torch.float16, i) for i in range(3)]
+        x, gate, res = (f[s:s + 700 * d].view(700, d) for f, s in zip(flat, shifts))
+        run_and_check(x, dict(gate=gate, residual=res, weight=rand(d, torch.float16, 9), next_weight=rand(d, torch.float16, 8)))
+
+
+def test_many_strided_rows():
+    base = rand((900, 3 * 256), torch.bfloat16, 1)
+    x, gate, res = base.split(256, dim=1)
+    w = rand(256, torch.bfloat16, 2)
+    run_and_check(x, dict(weight=w, gate=gate, residual=res, next_weight=w))
+    run_and_check(x, dict(weight=w, residual=res.contiguous()))
+    wide = rand((900, 4096 + 64), torch.float16, 3)
+    run_and_check(wide[:, :4096], dict(residual=wide[:, 64:], next_weight=rand(4096, torch.float32, 4)))
