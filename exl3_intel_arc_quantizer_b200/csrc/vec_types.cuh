@@ -141,6 +141,65 @@ __device__ __forceinline__ void store_piece(T* p, const float (&f)[V]) {
 }
 __device__ __forceinline__ void unpack(float x, float (&f)[1]) { f[0] = x; }
 
+// Arithmetic on V floats, two at a time where there are two (packed f32x2:
+// each lane rounds like the scalar operation)
+__device__ __forceinline__ float2 pair_of(float s) { return make_float2(s, s); }
+#define EXL3_PAIRWISE(a, pair_expr, one_expr)                              \
+  if constexpr (V % 2 == 0) {                                              \
+    _Pragma("unroll") for (int i = 0; i < V; i += 2) {                     \
+      const float2 x = make_float2((a)[i], (a)[i + 1]);                    \
+      const float2 r = pair_expr;                                          \
+      (a)[i] = r.x;                                                        \
+      (a)[i + 1] = r.y;                                                    \
+    }                                                                      \
+  } else {                                                                 \
+    _Pragma("unroll") for (int i = 0; i < V; ++i) {                        \
+      const float x = (a)[i];                                              \
+      (a)[i] = one_expr;                                                   \
+    }                                                                      \
+  }
+// a s
+template <int V>
+__device__ __forceinline__ void vec_scale(float (&a)[V], float s) {
+  EXL3_PAIRWISE(a, __fmul2_rn(x, pair_of(s)), x * s)
+}
+// a + s
+template <int V>
+__device__ __forceinline__ void vec_add(float (&a)[V], float s) {
+  EXL3_PAIRWISE(a, __fadd2_rn(x, pair_of(s)), x + s)
+}
+// a b
+template <int V>
+__device__ __forceinline__ void vec_mul(float (&a)[V], const float (&b)[V]) {
+  EXL3_PAIRWISE(a, __fmul2_rn(x, make_float2(b[i], b[i + 1])), x * b[i])
+}
+// s a + c
+template <int V>
+__device__ __forceinline__ void vec_axpy(float (&a)[V], float s, const float (&c)[V]) {
+  EXL3_PAIRWISE(a, __ffma2_rn(pair_of(s), x, make_float2(c[i], c[i + 1])), fmaf(s, x, c[i]))
+}
+// b a + c
+template <int V>
+__device__ __forceinline__ void vec_fma(float (&a)[V], const float (&b)[V], const float (&c)[V]) {
+  EXL3_PAIRWISE(a, __ffma2_rn(make_float2(b[i], b[i + 1]), x, make_float2(c[i], c[i + 1])),
+                fmaf(b[i], x, c[i]))
+}
+#undef EXL3_PAIRWISE
+// acc + a^2, two sums
+template <int V>
+__device__ __forceinline__ void vec_squares(const float (&a)[V], float2& acc) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 x = make_float2(a[i], a[i + 1]);
+      acc = __ffma2_rn(x, x, acc);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc.x = fmaf(a[i], a[i], acc.x);
+  }
+}
+
 inline bool aligned_to(const void* p, size_t bytes) {
   return reinterpret_cast<uintptr_t>(p) % bytes == 0;
 }
