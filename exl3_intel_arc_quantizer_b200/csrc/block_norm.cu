@@ -25,7 +25,10 @@ __device__ unsigned int g_norm_faults = 0;
 
 namespace {
 
-constexpr int kMaxThreads = 512;  // of a CTA that owns a row
+// Threads of a CTA that owns a row: three of 512 have 42 registers per thread.
+// 4,096 elements of 16 bits off a boundary are 513 vectors.
+constexpr int max_threads(bool shift) { return shift ? 544 : 512; }
+constexpr int max_warps(bool shift) { return (max_threads(shift) / 32 + 3) / 4 * 4; }  // whole 16 bytes
 
 __device__ __forceinline__ float act_sigmoid(float z) {
   float r;  // 2^-22; exp(-z) = inf gives 0
@@ -72,9 +75,9 @@ struct Held {
 // its elements c V - off .. c V - off + V - 1, the first and the last of them
 // moved element by element.
 template <typename T, typename P, int V, int NV, bool CTA_ROW, bool GATE, bool SHIFT>
-__global__ void __launch_bounds__(CTA_ROW ? kMaxThreads : 128, NV == 1 ? (CTA_ROW ? 4 : 16) : (CTA_ROW ? 2 : 8))
+__global__ void __launch_bounds__(CTA_ROW ? max_threads(SHIFT) : 128, NV == 1 ? (CTA_ROW ? 3 : 12) : (CTA_ROW ? 1 : 4))
 block_norm_kernel(const __grid_constant__ exl3_block_norm_args a, int lanes) {
-  constexpr int kRed = CTA_ROW ? kMaxThreads / 32 : 4;
+  constexpr int kRed = CTA_ROW ? max_warps(SHIFT) : 4;
   __shared__ __align__(16) float red[2][kRed];
   int side = 0;
   if (CTA_ROW) {
@@ -282,7 +285,7 @@ int launch(const exl3_block_norm_args& a, int threads, int lanes, cudaStream_t s
   const int per_cta = CTA_ROW ? 1 : threads / lanes;
   const int64_t ctas = (a.rows + per_cta - 1) / per_cta;
   // as many CTAs as run at once: each has a next row to load
-  static std::atomic<int> known[kMaxThreads / 32 + 1];  // by warps of a CTA
+  static std::atomic<int> known[max_threads(true) / 32 + 1];  // by warps of a CTA
   int resident = known[threads / 32].load(std::memory_order_relaxed);
   if (resident == 0) {
     EXL3_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, threads, 0));
@@ -307,10 +310,10 @@ int launch_v(const exl3_block_norm_args& a, cudaStream_t stream) {
     return launch<T, P, V, 4, false, GATE, SHIFT>(a, 128, lanes, stream);
   }
   const auto threads = [&](int nv) { return (int)((nvec + 32 * nv - 1) / (32 * nv)) * 32; };
-  if (nvec <= kMaxThreads)
+  if (nvec <= max_threads(SHIFT))
     return launch<T, P, V, 1, true, GATE, SHIFT>(a, threads(1), 32, stream);
-  if (nvec <= 2 * kMaxThreads) return launch<T, P, V, 2, true, GATE, SHIFT>(a, threads(2), 32, stream);
-  if (nvec <= 4 * kMaxThreads) return launch<T, P, V, 4, true, GATE, SHIFT>(a, threads(4), 32, stream);
+  if (nvec <= 2 * max_threads(SHIFT)) return launch<T, P, V, 2, true, GATE, SHIFT>(a, threads(2), 32, stream);
+  if (nvec <= 4 * max_threads(SHIFT)) return launch<T, P, V, 4, true, GATE, SHIFT>(a, threads(4), 32, stream);
   const int64_t most = (int64_t)sm_count() * 2;
   block_norm_long_kernel<T, P>
       <<<(unsigned)(a.rows < most ? a.rows : most), 1024, 0, stream>>>(a);

@@ -149,8 +149,8 @@ delta_tokens_kernel(const __grid_constant__ exl3_delta_args a, int vec) {
 
 template <typename T, bool STEP>
 int launch_tokens(const exl3_delta_args& a, cudaStream_t stream) {
-  const int cols = a.dk <= 128 ? 32 : 16;
-  const int64_t warps = a.seqs * a.heads * ((a.dv + cols - 1) / cols);
+  constexpr int kCols = 16;
+  const int64_t warps = a.seqs * a.heads * ((a.dv + kCols - 1) / kCols);
   const int64_t ctas = (warps + kWarps - 1) / kWarps;
   EXL3_REQUIRE(ctas < (1ll << 31), "too many sequences and heads");
   const auto fits = [](const void* p, const int64_t* st) {
@@ -158,9 +158,9 @@ int launch_tokens(const exl3_delta_args& a, cudaStream_t stream) {
   };
   const int vec = fits(a.q, a.q_strides) && fits(a.k, a.k_strides);
   if (a.dk <= 64)
-    delta_tokens_kernel<T, 16, 8, STEP><<<(unsigned)ctas, 32 * kWarps, 0, stream>>>(a, vec);
+    delta_tokens_kernel<T, 8, 4, STEP><<<(unsigned)ctas, 32 * kWarps, 0, stream>>>(a, vec);
   else if (a.dk <= 128)
-    delta_tokens_kernel<T, 32, 8, STEP><<<(unsigned)ctas, 32 * kWarps, 0, stream>>>(a, vec);
+    delta_tokens_kernel<T, 16, 4, STEP><<<(unsigned)ctas, 32 * kWarps, 0, stream>>>(a, vec);
   else
     delta_tokens_kernel<T, 32, 4, STEP><<<(unsigned)ctas, 32 * kWarps, 0, stream>>>(a, vec);
   EXL3_LAUNCHED();
