@@ -1198,7 +1198,7 @@ int launch_chunks(const exl3_delta_args& a, uint8_t* ws, cudaStream_t stream) {
                          stream>>>(a, ws, vec & 1);
   EXL3_LAUNCHED();
   const int64_t chains = a.seqs * a.heads;
-  if (chains * ((a.dv + 31) / 32) <= sm_count())
+  if (chains * ((a.dv + 31) / 32) <= 2 * sm_count())
     return launch_chain<T, 1, 32, 16>(a, ws, vec, stream);
   return launch_chain<T, 2, 64, 32>(a, ws, vec, stream);
 }
