@@ -117,7 +117,7 @@ __device__ __forceinline__ uint4 load8(const T* p, bool vec) {
 // ---------------------------------------------------------------------------
 
 constexpr int kPrepThreads = 256;
-constexpr int kPrepHeads = 8;  // heads whose gates are prepared at once
+constexpr int kPrepHeads = 4;  // heads whose gates are prepared at once
 constexpr int kLds = 68;       // floats per row of the 64 x 64 matrices
 
 // What depends on a head's g and beta. R_b is the prefix sum before block b
@@ -129,26 +129,34 @@ struct alignas(16) Gates {
   float down[3][48];         // 2^(R_b - G_j), b = 1..3, j < 16 b
   float beta[kChunk];
   float total[2];            // G_63 / ln 2 in two parts
+  float grow;                // 2 to the sum of the positive g / ln 2: no decay is above it
 };
 
 struct PrepSmem {
-  uint8_t kq[kKqBytes];      // the chain's [K; Q]; later P T's two parts
+  union {
+    uint8_t kq[kKqBytes];               // the chain's [K; Q]
+    float4 dots[8][kPrepThreads];       // then each thread's part of K K^T or Q K^T
+  } a;
   union {
     float M[kChunk][kLds];
-    uint8_t t[2][kChunk * 128];  // T's two parts, when M has been used
+    uint8_t t[2][kChunk * 128];         // T's two parts, when M has been used
   } m;
-  float X[kChunk][kLds];
-  float tmp[32][36];
+  union {
+    // (I + M)^-1; its upper right quadrant, which is zero, holds the products
+    // on the way
+    float X[kChunk][kLds];
+    uint8_t pt[2][kChunk * 128];        // P T's two parts, when X has been used
+  } x;
   Gates gates[kPrepHeads];
-  // of row i: the power of two on its way to fp16 and back, and the factor
-  // 1 / |.| (1 where rows are taken as they are)
+  // of row i: the power of two on its way to fp16 and back, the factor
+  // 1 / |.| (1 where rows are taken as they are), and |.|
   float back[2 * kChunk], unit[2 * kChunk], norm[kChunk];
-  uint32_t peak[3];          // bits of max |T|, max |P T|, largest row sum of |T|
+  uint32_t most[2];          // bits of the largest unit |k| and unit |q|
+  uint32_t peak[2];          // bits of max |T| and of the largest row sum of |T|
 };
 
 static_assert(sizeof(Gates) % 16 == 0 && offsetof(Gates, g) % 16 == 0 && offsetof(Gates, beta) % 16 == 0 &&
-                  offsetof(PrepSmem, m) % 16 == 0 && offsetof(PrepSmem, X) % 16 == 0 &&
-                  offsetof(PrepSmem, tmp) % 16 == 0 &&
+                  offsetof(PrepSmem, m) % 16 == 0 && offsetof(PrepSmem, x) % 16 == 0 &&
                   offsetof(PrepSmem, gates) % 16 == 0 && offsetof(PrepSmem, back) % 16 == 0 &&
                   kLds % 4 == 0,
               "16-byte accesses");
@@ -160,6 +168,43 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
       "{%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// fp32 products on the tensor cores: each factor as two tf32 parts (22 bits),
+// the product of the low ones left out
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
+}
+__device__ __forceinline__ void mma1688(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+// A warp's 16 x 8 block of left (16 x K) right (K x 8), rows of kLds floats
+template <int K>
+__device__ __forceinline__ void block_product(const float* left, const float* right, int lane, float (&c)[4]) {
+  const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c[e] = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; k += 8) {
+    uint32_t ah[4], al[4], bh[2], bl[2];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      split_tf32(left[(g + 8 * (e & 1)) * kLds + k + t + 4 * (e >> 1)], ah[e], al[e]);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) split_tf32(right[(k + t + 4 * e) * kLds + g], bh[e], bl[e]);
+    mma1688(c, ah, bl);
+    mma1688(c, al, bh);
+    mma1688(c, ah, bh);
+  }
+}
+__device__ __forceinline__ void store_block(float* to, int lane, const float (&c)[4], float sign) {
+  const int g = lane >> 2, t = lane & 3;
+  *reinterpret_cast<float2*>(to + g * kLds + 2 * t) = make_float2(sign * c[0], sign * c[1]);
+  *reinterpret_cast<float2*>(to + (g + 8) * kLds + 2 * t) = make_float2(sign * c[2], sign * c[3]);
 }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -177,10 +222,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 // One CTA per chunk and key head. Bound by instruction issue and the latency
-// of the inverse's steps (two CTAs share an SM); the reads and writes are
+// of the inverse's steps (three CTAs share an SM); the reads and writes are
 // 64 KB per key head and 33 KB per head.
 template <typename T>
-__global__ void __launch_bounds__(kPrepThreads, 2)
+__global__ void __launch_bounds__(kPrepThreads, 3)
 delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict__ ws, int vec) {
   extern __shared__ __align__(128) uint8_t prep_smem[];
   PrepSmem& sm = *reinterpret_cast<PrepSmem*>(prep_smem);
@@ -202,6 +247,8 @@ delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict
   if (t0 >= t1) return;
   const int n = (int)(t1 - t0 < kChunk ? t1 - t0 : kChunk);
   uint8_t* const out = ws + slot * slot_bytes(a);
+  if (tid < 2) sm.most[tid] = 0;
+  __syncthreads();
 
   // [K; Q] in fp16, zeros past the chunk's end and past dk: 16 neighbouring
   // threads hold a row, a thread one 16-byte piece of eight rows
@@ -243,7 +290,7 @@ delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict
         x[i] = make_uint4(w[0], w[1], w[2], w[3]);
       }
       const uint32_t at = (q >> 3) * (kKqBytes / 2) + swz(r, q & 7);
-      *reinterpret_cast<uint4*>(sm.kq + at) = x[i];
+      *reinterpret_cast<uint4*>(sm.a.kq + at) = x[i];
       *reinterpret_cast<uint4*>(out + (int64_t)kh * kKqBytes + at) = x[i];
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss = fmaf(f[j], f[j], ss);
@@ -252,24 +299,27 @@ delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict
       if (q == 0) {
         sm.back[r] = back;
         // 1 / sqrt(|x|^2 + eps) with x = back times what was summed
-        sm.unit[r] = a.normalize_qk ? rsqrtf(fmaf(ss * back, back, kNormEps)) : 1.f;
-        if (i < 4) sm.norm[r] = sqrtf(ss) * back;
+        const float unit = a.normalize_qk ? rsqrtf(fmaf(ss * back, back, kNormEps)) : 1.f;
+        const float norm = sqrtf(ss) * back;
+        sm.unit[r] = unit;
+        if (i < 4) sm.norm[r] = norm;
+        atomicMax(&sm.most[i >> 2], __float_as_uint(unit * norm));
       }
     }
   }
   __syncthreads();
 
   // warps 0-3: rows 16 mt of K K^T; warps 4-7: of Q K^T; columns up to the
-  // diagonal tile. They stay in registers for all heads.
+  // diagonal tile. Kept for all heads where [K; Q] was.
   const int mt = warp & 3, which = warp >> 2;
-  float acc[8][4];
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
   {
+    float acc[8][4];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
     const auto at = [&](int r, int piece) {
-      return smem_u32(sm.kq + (piece >> 3) * (kKqBytes / 2) + swz(r, piece & 7));
+      return smem_u32(sm.a.kq + (piece >> 3) * (kKqBytes / 2) + swz(r, piece & 7));
     };
     for (int k = 0; k < (a.dk + 15) / 16; ++k) {
       uint32_t fa[4];
@@ -283,6 +333,11 @@ delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict
         mma16816(acc[2 * j + 1], fa, fb[2], fb[3]);
       }
     }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j <= 2 * mt + 1)
+        sm.a.dots[j][tid] = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
   }
   const int r0 = 16 * mt + (lane >> 2), c0 = 2 * (lane & 3);  // of a fragment's first element
 
@@ -293,7 +348,8 @@ delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict
     float* const vecs = reinterpret_cast<float*>(img + kImageBytes);
     if (h % kPrepHeads == 0) {
       if (h) __syncthreads();
-      if (h + warp < rep) {
+      static_assert(kPrepHeads <= kPrepThreads / 32, "a warp per head");
+      if (warp < kPrepHeads && h + warp < rep) {
         // a warp per head: prefix sums in fp64
         Gates& gt = sm.gates[warp];
         double g[2], run;
@@ -328,7 +384,11 @@ delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict
           for (int i = 0; i < 2; ++i)
             if (2 * lane + i < 16 * b) gt.down[b - 1][2 * lane + i] = exp2_fast((float)(Rb - G[i]));
         }
+        double pos = fmax(g[0], 0.0) + fmax(g[1], 0.0);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) pos += __shfl_xor_sync(0xFFFFFFFFu, pos, o);
         if (lane == 31) {
+          gt.grow = exp2f((float)pos) * 1.001f;
           const float hi = (float)run;
           gt.total[0] = hi;
           gt.total[1] = (float)(run - (double)hi);
@@ -337,78 +397,71 @@ delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict
       __syncthreads();
     }
     const Gates& gt = sm.gates[h % kPrepHeads];
-    if (tid < 3) sm.peak[tid] = 0;
+    if (tid < 2) sm.peak[tid] = 0;
 
     // M into shared memory; P as the first operand of P T, in two fp16 parts
-    // under the warp's scale
+    // under a scale from |P_ij| <= |scale| |q_i| |k_j| (no decay above grow)
     uint32_t ph[4][4], pl[4][4];
-    float inv_p = 1.f;
+    const float bound_p =
+        fabsf(a.scale) * __uint_as_float(sm.most[0]) * __uint_as_float(sm.most[1]) * gt.grow * 1.001f;
+    float scale_p, inv_p;
+    pow2_scale(bound_p, scale_p, inv_p);
     {
-      float f[8][4];
       float row[2], up[2];
       float2 gr[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int r = r0 + 8 * i;
-        row[i] = which ? a.scale * sm.unit[64 + r] * sm.back[64 + r] : gt.beta[r] * sm.unit[r] * sm.back[r];
+        row[i] = which ? a.scale * scale_p * sm.unit[64 + r] * sm.back[64 + r]
+                       : gt.beta[r] * sm.unit[r] * sm.back[r];
         up[i] = row[i] * gt.up[r];
         gr[i] = gt.g[r];
       }
-      float most = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
+        float f[4] = {0.f, 0.f, 0.f, 0.f};
+        if (j <= 2 * mt + 1) {
+          const int c = 8 * j + c0;
+          const float2 u = *reinterpret_cast<const float2*>(&sm.unit[c]);
+          const float2 bk = *reinterpret_cast<const float2*>(&sm.back[c]);
+          const float4 dot = sm.a.dots[j][tid];
+          float2 col = make_float2(u.x * bk.x, u.y * bk.y);
+          if (j < 2 * mt) {
+            const float2 dn = *reinterpret_cast<const float2*>(&gt.down[mt - 1][c]);
+            col.x *= dn.x;
+            col.y *= dn.y;
+            f[0] = dot.x * col.x * up[0];
+            f[1] = dot.y * col.y * up[0];
+            f[2] = dot.z * col.x * up[1];
+            f[3] = dot.w * col.y * up[1];
+          } else {
+            const float4 gc = *reinterpret_cast<const float4*>(&gt.g[c]);
+            const float v[4] = {dot.x, dot.y, dot.z, dot.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f[j][e] = 0.f;
-        if (j > 2 * mt + 1) continue;
-        const int c = 8 * j + c0;
-        const float2 u = *reinterpret_cast<const float2*>(&sm.unit[c]);
-        const float2 bk = *reinterpret_cast<const float2*>(&sm.back[c]);
-        float2 col = make_float2(u.x * bk.x, u.y * bk.y);
-        if (j < 2 * mt) {
-          const float2 dn = *reinterpret_cast<const float2*>(&gt.down[mt - 1][c]);
-          col.x *= dn.x;
-          col.y *= dn.y;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            f[j][2 * i] = acc[j][2 * i] * col.x * up[i];
-            f[j][2 * i + 1] = acc[j][2 * i + 1] * col.y * up[i];
+            for (int i = 0; i < 2; ++i) {
+              const int last = which ? r0 + 8 * i : r0 + 8 * i - 1;  // P has its diagonal
+              const float d0 = exp2_fast((gr[i].x - gc.x) + (gr[i].y - gc.y));
+              const float d1 = exp2_fast((gr[i].x - gc.z) + (gr[i].y - gc.w));
+              f[2 * i] = c <= last ? v[2 * i] * col.x * row[i] * d0 : 0.f;
+              f[2 * i + 1] = c + 1 <= last ? v[2 * i + 1] * col.y * row[i] * d1 : 0.f;
+            }
           }
-        } else {
-          const float4 gc = *reinterpret_cast<const float4*>(&gt.g[c]);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int r = r0 + 8 * i;
-            const float d0 = exp2_fast((gr[i].x - gc.x) + (gr[i].y - gc.y));
-            const float d1 = exp2_fast((gr[i].x - gc.z) + (gr[i].y - gc.w));
-            const int last = which ? r : r - 1;  // P has its diagonal
-            f[j][2 * i] = c <= last ? acc[j][2 * i] * col.x * row[i] * d0 : 0.f;
-            f[j][2 * i + 1] = c + 1 <= last ? acc[j][2 * i + 1] * col.y * row[i] * d1 : 0.f;
+          if (!which) {
+            *reinterpret_cast<float2*>(&sm.m.M[r0][c]) = make_float2(f[0], f[1]);
+            *reinterpret_cast<float2*>(&sm.m.M[r0 + 8][c]) = make_float2(f[2], f[3]);
           }
         }
+        // rows r0 and r0 + 8 of columns 8 j .. are registers 2 (j & 1) and the next
         if (which) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(f[j][e]));
-        } else {
-          *reinterpret_cast<float2*>(&sm.m.M[r0][c]) = make_float2(f[j][0], f[j][1]);
-          *reinterpret_cast<float2*>(&sm.m.M[r0 + 8][c]) = make_float2(f[j][2], f[j][3]);
+          split2(make_float2(f[0], f[1]), ph[j >> 1][2 * (j & 1)], pl[j >> 1][2 * (j & 1)]);
+          split2(make_float2(f[2], f[3]), ph[j >> 1][2 * (j & 1) + 1], pl[j >> 1][2 * (j & 1) + 1]);
         }
-      }
-      if (which) {
-        most = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most)));
-        float scale;
-        pow2_scale(most, scale, inv_p);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float* v = &f[2 * k + (e >> 1)][2 * (e & 1)];
-            split2(make_float2(v[0] * scale, v[1] * scale), ph[k][e], pl[k][e]);
-          }
       }
     }
     __syncthreads();
     float(&M)[kChunk][kLds] = sm.m.M;
-    float(&X)[kChunk][kLds] = sm.X;
+    float(&X)[kChunk][kLds] = sm.x.X;
+    float* const tmp = &X[0][32];  // 32 x 32
     // (I + M)^-1: the 16x16 diagonal blocks, a thread per column
     if (tid < 64) {
       const int b = tid & ~15, c = tid & 15;
@@ -430,58 +483,34 @@ delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict
       for (int i = 0; i < 16; ++i) X[b + i][b + c] = x[i];
     }
     __syncthreads();
-    // halves of 32: X21 = -X22 (M21 X11), two pairs of blocks at once
+    // halves of 32: X21 = -X22 (M21 X11), two pairs of blocks, a warp for eight
+    // columns; the other warps clear the blocks above the diagonal
     {
-      const int p = tid >> 7, r = (tid >> 3) & 15, c = 2 * (tid & 7), b = 32 * p;
-      float2 v = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int k = 0; k < 16; k += 4) {
-        const float4 m = *reinterpret_cast<const float4*>(&M[b + 16 + r][b + k]);
-        v = __ffma2_rn(make_float2(m.x, m.x), *reinterpret_cast<const float2*>(&X[b + k][b + c]), v);
-        v = __ffma2_rn(make_float2(m.y, m.y), *reinterpret_cast<const float2*>(&X[b + k + 1][b + c]), v);
-        v = __ffma2_rn(make_float2(m.z, m.z), *reinterpret_cast<const float2*>(&X[b + k + 2][b + c]), v);
-        v = __ffma2_rn(make_float2(m.w, m.w), *reinterpret_cast<const float2*>(&X[b + k + 3][b + c]), v);
+      const int b = 32 * ((warp >> 1) & 1), c = 8 * (warp & 1);
+      float v[4];
+      if (warp < 4) {
+        block_product<16>(&M[b + 16][b], &X[b][b + c], lane, v);
+        store_block(tmp + (b >> 1) * kLds + c, lane, v, 1.f);
+      } else {
+        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+        store_block(&X[b][b + 16 + c], lane, zero, 1.f);
       }
-      *reinterpret_cast<float2*>(&sm.tmp[16 * p + r][c]) = v;
       __syncthreads();
-      v = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int k = 0; k < 16; k += 4) {
-        const float4 m = *reinterpret_cast<const float4*>(&X[b + 16 + r][b + 16 + k]);
-        const float* w = &sm.tmp[16 * p + k][c];
-        v = __ffma2_rn(make_float2(m.x, m.x), *reinterpret_cast<const float2*>(w), v);
-        v = __ffma2_rn(make_float2(m.y, m.y), *reinterpret_cast<const float2*>(w + 36), v);
-        v = __ffma2_rn(make_float2(m.z, m.z), *reinterpret_cast<const float2*>(w + 72), v);
-        v = __ffma2_rn(make_float2(m.w, m.w), *reinterpret_cast<const float2*>(w + 108), v);
+      if (warp < 4) {
+        block_product<16>(&X[b + 16][b + 16], tmp + (b >> 1) * kLds + c, lane, v);
+        store_block(&X[b + 16][b + c], lane, v, -1.f);
       }
-      *reinterpret_cast<float2*>(&X[b + 16 + r][b + c]) = make_float2(-v.x, -v.y);
-      // the blocks above the diagonal of X11 and X22
-      *reinterpret_cast<float2*>(&X[b + r][b + 16 + c]) = make_float2(0.f, 0.f);
     }
     __syncthreads();
     // the whole: the same with blocks of 32
     {
-      const int r = tid >> 3, c = 4 * (tid & 7);
-      float2 v[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      const auto product = [&](const float* left, const float* right, int pitch) {
-#pragma unroll
-        for (int k = 0; k < 32; k += 4) {
-          const float4 m = *reinterpret_cast<const float4*>(left + k);
-          const float w[4] = {m.x, m.y, m.z, m.w};
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            const float4 x = *reinterpret_cast<const float4*>(right + (k + kk) * pitch);
-            v[0] = __ffma2_rn(make_float2(w[kk], w[kk]), make_float2(x.x, x.y), v[0]);
-            v[1] = __ffma2_rn(make_float2(w[kk], w[kk]), make_float2(x.z, x.w), v[1]);
-          }
-        }
-      };
-      product(&M[32 + r][0], &X[0][c], kLds);
-      *reinterpret_cast<float4*>(&sm.tmp[r][c]) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+      const int r = 16 * (warp >> 2), c = 8 * (warp & 3);
+      float v[4];
+      block_product<32>(&M[32 + r][0], &X[0][c], lane, v);
+      store_block(tmp + r * kLds + c, lane, v, 1.f);
       __syncthreads();
-      v[0] = v[1] = make_float2(0.f, 0.f);
-      product(&X[32 + r][32], &sm.tmp[0][c], 36);
-      *reinterpret_cast<float4*>(&X[32 + r][c]) = make_float4(-v[0].x, -v[0].y, -v[1].x, -v[1].y);
+      block_product<32>(&X[32 + r][32], tmp + c, lane, v);
+      store_block(&X[32 + r][c], lane, v, -1.f);
     }
     __syncthreads();
     // T = X beta: 16 columns of a row per thread, its peak and row sums
@@ -510,7 +539,7 @@ delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict
       const uint32_t m2 = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(sum));
       if (lane == 0) {
         atomicMax(&sm.peak[0], m0);
-        atomicMax(&sm.peak[2], m2);
+        atomicMax(&sm.peak[1], m2);
       }
       __syncthreads();
       float scale, inv;
@@ -530,60 +559,50 @@ delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict
     }
     __syncthreads();
     if (which) {
-      // P T, rows of this warp: three products of parts per 16 x 16 block
-      float o[8][4];
+      // P T, rows of this warp: three products of parts per 16 x 16 block; its
+      // scale from |P T| <= 64 max |P| max |T|
+      const float max_t = __uint_as_float(sm.peak[0]);
+      float scale_t, inv_t, scale, inv;
+      pow2_scale(max_t, scale_t, inv_t);
+      pow2_scale(64.f * bound_p * max_t, scale, inv);
+      const float f = inv_p * inv_t * scale;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int j = 0; j < 4; ++j) {
+        float o[2][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
+        for (int e = 0; e < 8; ++e) o[e >> 2][e & 3] = 0.f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (k > mt) break;
-#pragma unroll
-        for (int j = 0; j <= k; ++j) {
+        for (int k = 0; k < 4; ++k) {
+          if (k < j || k > mt) continue;
           const uint32_t at = swz(16 * k + (lane & 15), 2 * j + (lane >> 4));
           uint32_t bh[4], bl[4];
           ldsm4_trans(bh, smem_u32(sm.m.t[0] + at));
           ldsm4_trans(bl, smem_u32(sm.m.t[1] + at));
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            mma16816(o[2 * j + e], ph[k], bh[2 * e], bh[2 * e + 1]);
-            mma16816(o[2 * j + e], ph[k], bl[2 * e], bl[2 * e + 1]);
-            mma16816(o[2 * j + e], pl[k], bh[2 * e], bh[2 * e + 1]);
+            mma16816(o[e], ph[k], bh[2 * e], bh[2 * e + 1]);
+            mma16816(o[e], ph[k], bl[2 * e], bl[2 * e + 1]);
+            mma16816(o[e], pl[k], bh[2 * e], bh[2 * e + 1]);
           }
         }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t hi, lo;
+            split2(make_float2(o[e][2 * i] * f, o[e][2 * i + 1] * f), hi, lo);
+            const uint32_t at = swz(r0 + 8 * i, 2 * j + e) + 2 * c0;
+            *reinterpret_cast<uint32_t*>(sm.x.pt[0] + at) = hi;
+            *reinterpret_cast<uint32_t*>(sm.x.pt[1] + at) = lo;
+          }
       }
-      float scale, inv, most = 0.f;
-      pow2_scale(__uint_as_float(sm.peak[0]), scale, inv);
-      inv *= inv_p;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          o[j][e] *= inv;
-          most = fmaxf(most, fabsf(o[j][e]));
-        }
-      const uint32_t m1 = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most));
-      if (lane == 0) atomicMax(&sm.peak[1], m1);
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      pow2_scale(__uint_as_float(sm.peak[1]), scale, inv);
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t hi, lo;
-          split2(make_float2(o[j][2 * i] * scale, o[j][2 * i + 1] * scale), hi, lo);
-          const uint32_t at = swz(r0 + 8 * i, j) + 2 * c0;
-          *reinterpret_cast<uint32_t*>(sm.kq + at) = hi;
-          *reinterpret_cast<uint32_t*>(sm.kq + kChunk * 128 + at) = lo;
-        }
       if (tid == 128) vecs[kScalePT] = inv;
       asm volatile("bar.sync 1, 128;" ::: "memory");
       // rows 64-127 of the image's two tiles
       for (int i = tid - 128; i < 2 * kChunk * 8; i += 128) {
         const int part = i >> 9, at = (i & 511) * 16;
         *reinterpret_cast<uint4*>(img + part * (kImageBytes / 2) + kChunk * 128 + at) =
-            *reinterpret_cast<const uint4*>(sm.kq + part * (kChunk * 128) + at);
+            *reinterpret_cast<const uint4*>(sm.x.pt[part] + at);
       }
     } else if (warp == 0) {
       float ba = 0.f, bu = 0.f, bs = 0.f;
@@ -607,7 +626,7 @@ delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict
         bs += __shfl_xor_sync(0xFFFFFFFFu, bs, o);
       }
       if (lane == 0) {
-        const float t = __uint_as_float(sm.peak[2]);
+        const float t = __uint_as_float(sm.peak[1]);
         float scale, inv;
         pow2_scale(__uint_as_float(sm.peak[0]), scale, inv);
         vecs[kGamma] = exp2_fast(gt.total[0] + gt.total[1]);
