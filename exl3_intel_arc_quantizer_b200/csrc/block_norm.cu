@@ -13,16 +13,10 @@
 // next row's vectors before they work on this one's, so that loads are in
 // flight across the sums; rows past the registers of a CTA are read again for
 // each sum.
-#include <algorithm>
-
 #include "common.cuh"
-#include "pipeline.cuh"
 #include "vec_types.cuh"
 
 namespace exl3 {
-
-__device__ unsigned int g_norm_faults = 0;
-
 namespace {
 
 // Threads of a CTA that owns a row: three of 512 have 42 registers per thread.
@@ -348,11 +342,6 @@ int launch_t(const exl3_block_norm_args& a, cudaStream_t stream) {
 }
 
 }  // namespace
-
-int norm_fault_count(unsigned int* count) {
-  EXL3_CUDA(cudaMemcpyFromSymbol(count, g_norm_faults, sizeof(unsigned int)));
-  return EXL3_OK;
-}
 
 }  // namespace exl3
 

@@ -1236,12 +1236,9 @@ int delta_chunks(const exl3_delta_args& a, void* ws, cudaStream_t stream) {
 
 }  // namespace exl3
 
-extern "C" int exl3_layer_fault_count(unsigned int* count) {
+extern "C" int exl3_delta_fault_count(unsigned int* count) {
   using namespace exl3;
   EXL3_REQUIRE(count != nullptr, "count is NULL");
-  unsigned int delta = 0, norm = 0;
-  EXL3_CUDA(cudaMemcpyFromSymbol(&delta, g_delta_faults, sizeof(unsigned int)));
-  if (const int rc = norm_fault_count(&norm)) return rc;
-  *count = delta + norm;
+  EXL3_CUDA(cudaMemcpyFromSymbol(count, g_delta_faults, sizeof(unsigned int)));
   return EXL3_OK;
 }

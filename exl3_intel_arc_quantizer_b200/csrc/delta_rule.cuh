@@ -12,8 +12,6 @@ constexpr float kNormEps = 1e-6f;  // added to a sum of squares of q or k
 size_t delta_chunk_ws_bytes(const exl3_delta_args& a);
 int delta_chunks(const exl3_delta_args& a, void* ws, cudaStream_t stream);
 
-int norm_fault_count(unsigned int* count);  // block_norm.cu
-
 // Tokens [t0, t1) of sequence s. The offsets are device data that the host
 // has not seen: they are clamped into [0, tokens], and a sequence that would
 // end before it begins is empty.

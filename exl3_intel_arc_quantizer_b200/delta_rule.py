@@ -11,11 +11,12 @@ Per value head, with the state S (dk, dv) in fp32::
 
 from __future__ import annotations
 
+import ctypes
 from typing import Optional, Tuple
 
 import torch
 
-from ._ext import ext, require_cuda
+from ._ext import _check, ext, lib, require_cuda
 
 
 def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor,
@@ -87,3 +88,13 @@ def gated_delta_step_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torc
         require_cuda(q.device)
     return ext().gated_delta_step_(q, k, v, g, beta, state, slots,
                                    q.shape[-1] ** -0.5 if scale is None else scale, normalize_qk)
+
+
+def delta_fault_count() -> int:
+    """CTAs of the delta rule's whole-sequence kernel that gave up a
+    bounded wait (2 s) on the current device since the library loaded
+    (``exl3_delta_fault_count``; 0 when every call was valid). Synchronizes the
+    device."""
+    n = ctypes.c_uint(0)
+    _check(lib().exl3_delta_fault_count(ctypes.byref(n)))
+    return int(n.value)

@@ -1,0 +1,187 @@
+"""Hybrid decoder layers for calibration on B200: gated linear attention and
+rotary softmax attention around the same MLP.
+
+``calibration.hessian_groups`` names the projections of a linear-attention
+layer (``linear_attn.in_proj_qkv / in_proj_z / in_proj_b / in_proj_a`` share
+an input, ``linear_attn.out_proj`` has its own); the reference builds such
+layers from another library (``exl3_quant/hybrid.py:170-256``). The layers here
+run what lies between the projections on this package's kernels: the gated
+delta rule (``delta_rule``), rotary positions (``rotary``) and the norms with
+their gates and residual sums (``norms``). ``converter.convert_layer`` takes
+them with ``layer_runner=run_layer``::
+
+    layer = HybridDecoderLayer(4096, 12288, linear=True)
+    results, hidden, timings = convert_layer(layer, hidden, K=4, layer_runner=run_layer,
+                                             module_names=layer.quantizable())
+
+``HybridDecoderLayer.step`` runs a linear layer one token at a time from a
+:class:`LinearCache`, as a generation check of a converted layer does.
+"""
+
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+from typing import List, Optional, Tuple
+
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+from .calibration import DEFAULT_RMS_NORM_EPS, LlamaMLP, enumerate_linear_modules
+from .delta_rule import gated_delta_rule, gated_delta_step_
+from .norms import block_norm
+from .rotary import apply_rotary, rotary_frequencies
+
+
+@dataclass
+class LinearCache:
+    """A linear layer's memory of its sequences: the last inputs of the short
+    convolution (batch, channels, width - 1) and the states (batch, heads, dk,
+    dv)."""
+    conv: torch.Tensor
+    state: torch.Tensor
+
+
+class GatedDeltaAttention(nn.Module):
+    def __init__(self, hidden_size: int, key_heads: int = 16, heads: int = 32, key_dim: int = 128,
+                 value_dim: int = 128, conv_width: int = 4, eps: float = DEFAULT_RMS_NORM_EPS):
+        super().__init__()
+        if heads % key_heads:
+            raise ValueError(f"heads ({heads}) must be a multiple of key_heads ({key_heads})")
+        self.key_heads, self.heads, self.key_dim, self.value_dim = key_heads, heads, key_dim, value_dim
+        self.sizes = [key_heads * key_dim, key_heads * key_dim, heads * value_dim]
+        self.eps = eps
+        self.in_proj_qkv = nn.Linear(hidden_size, sum(self.sizes), bias=False)
+        self.in_proj_z = nn.Linear(hidden_size, heads * value_dim, bias=False)
+        self.in_proj_b = nn.Linear(hidden_size, heads, bias=False)
+        self.in_proj_a = nn.Linear(hidden_size, heads, bias=False)
+        self.out_proj = nn.Linear(heads * value_dim, hidden_size, bias=False)
+        self.conv_weight = nn.Parameter(torch.randn(sum(self.sizes), 1, conv_width) / conv_width ** 0.5)
+        self.A_log = nn.Parameter(torch.empty(heads).uniform_(0.01, 16).log())
+        self.dt_bias = nn.Parameter(torch.empty(heads).uniform_(-6.9, -2.3))
+        self.norm_weight = nn.Parameter(torch.ones(value_dim))
+
+    def _gates(self, x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        rate = -self.A_log.float().exp()
+        g = rate * F.softplus(self.in_proj_a(x).float() + self.dt_bias.float())
+        return g, torch.sigmoid(self.in_proj_b(x).float())
+
+    def _heads(self, mixed: torch.Tensor):
+        q, k, v = mixed.split(self.sizes, dim=-1)
+        return (q.unflatten(-1, (self.key_heads, self.key_dim)), k.unflatten(-1, (self.key_heads, self.key_dim)),
+                v.unflatten(-1, (self.heads, self.value_dim)))
+
+    def _out(self, o: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
+        z = self.in_proj_z(x).unflatten(-1, (self.heads, self.value_dim))
+        y, _ = block_norm(o, weight=self.norm_weight, gate=z, eps=self.eps)
+        return self.out_proj(y.flatten(-2))
+
+    def forward(self, x: torch.Tensor, cache: Optional[LinearCache] = None
+                ) -> Tuple[torch.Tensor, LinearCache]:
+        """x (batch, tokens, hidden), from a cache or from nothing."""
+        width = self.conv_weight.shape[-1]
+        raw = self.in_proj_qkv(x).transpose(1, 2)
+        if cache is None:
+            raw = F.pad(raw, (width - 1, 0))
+        else:
+            raw = torch.cat((cache.conv, raw), dim=-1)
+        mixed = F.silu(F.conv1d(raw, self.conv_weight, groups=raw.shape[1])).transpose(1, 2).contiguous()
+        g, beta = self._gates(x)
+        o, state = gated_delta_rule(*self._heads(mixed), g, beta, normalize_qk=True,
+                                    initial_state=None if cache is None else cache.state)
+        return self._out(o, x), LinearCache(raw[..., raw.shape[-1] - width + 1:].contiguous(), state)
+
+    def step(self, x: torch.Tensor, cache: LinearCache) -> torch.Tensor:
+        """x (batch, hidden): one token of each sequence; the cache moves on."""
+        raw = torch.cat((cache.conv, self.in_proj_qkv(x)[..., None]), dim=-1)
+        mixed = F.silu((raw.float() * self.conv_weight[:, 0].float()).sum(-1)).to(x.dtype)
+        cache.conv.copy_(raw[..., 1:])
+        g, beta = self._gates(x)
+        o = gated_delta_step_(*self._heads(mixed), g, beta, cache.state, normalize_qk=True)
+        return self._out(o, x)
+
+
+class RotaryAttention(nn.Module):
+    """Causal softmax attention with rotary positions on part of the head."""
+
+    def __init__(self, hidden_size: int, heads: int = 32, kv_heads: int = 8, head_dim: int = 128,
+                 rotary_dim: Optional[int] = None, interleaved: bool = False, **frequencies):
+        super().__init__()
+        self.heads, self.kv_heads, self.head_dim, self.interleaved = heads, kv_heads, head_dim, interleaved
+        self.q_proj = nn.Linear(hidden_size, heads * head_dim, bias=False)
+        self.k_proj = nn.Linear(hidden_size, kv_heads * head_dim, bias=False)
+        self.v_proj = nn.Linear(hidden_size, kv_heads * head_dim, bias=False)
+        self.o_proj = nn.Linear(heads * head_dim, hidden_size, bias=False)
+        # not a buffer: a layer's conversion to fp16 must not round it
+        self.inv_freq, self.attention_factor = rotary_frequencies(rotary_dim or head_dim, **frequencies)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        b, s, _ = x.shape
+        if self.inv_freq.device != x.device:
+            self.inv_freq = self.inv_freq.to(x.device)
+        q = self.q_proj(x).view(b, s, self.heads, self.head_dim).transpose(1, 2)
+        k = self.k_proj(x).view(b, s, self.kv_heads, self.head_dim).transpose(1, 2)
+        v = self.v_proj(x).view(b, s, self.kv_heads, self.head_dim).transpose(1, 2)
+        q, k = apply_rotary(q, k, torch.arange(s, device=x.device), self.inv_freq,
+                            attention_factor=self.attention_factor, interleaved=self.interleaved,
+                            heads_first=True)
+        rep = self.heads // self.kv_heads
+        k, v = k.repeat_interleave(rep, 1), v.repeat_interleave(rep, 1)
+        att = torch.matmul(q, k.transpose(-2, -1)).float() / math.sqrt(self.head_dim)
+        late = torch.ones(s, s, dtype=torch.bool, device=x.device).triu(1)
+        att = att.masked_fill(late, -math.inf).softmax(-1).to(q.dtype)
+        return self.o_proj(torch.matmul(att, v).transpose(1, 2).reshape(b, s, -1))
+
+
+class HybridDecoderLayer(nn.Module):
+    """norm, attention of either kind (``linear_attn`` or ``self_attn``),
+    residual sum and norm in one pass, MLP, residual sum. Runs under
+    ``torch.no_grad()``, as calibration does."""
+
+    def __init__(self, hidden_size: int, intermediate_size: int, linear: bool,
+                 eps: float = DEFAULT_RMS_NORM_EPS, **attention):
+        super().__init__()
+        self.eps = eps
+        if linear:
+            self.linear_attn = GatedDeltaAttention(hidden_size, eps=eps, **attention)
+        else:
+            self.self_attn = RotaryAttention(hidden_size, **attention)
+        self.input_norm = nn.Parameter(torch.ones(hidden_size))
+        self.post_attention_norm = nn.Parameter(torch.ones(hidden_size))
+        self.mlp = LlamaMLP(hidden_size, intermediate_size)
+
+    def quantizable(self) -> List[str]:
+        """The projections that the quantizer takes: in and out features in
+        whole blocks of 128 (the two gate projections of a linear layer have
+        one output per head and stay as they are)."""
+        return [name for name, m in enumerate_linear_modules(self).items()
+                if m.in_features % 128 == 0 and m.out_features % 128 == 0]
+
+    def _after(self, mixed: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
+        h, n = block_norm(mixed, residual=x, next_weight=self.post_attention_norm, eps=self.eps)
+        return block_norm(self.mlp(n), residual=h)[0]
+
+    def forward(self, x: torch.Tensor, cache: Optional[LinearCache] = None
+                ) -> Tuple[torch.Tensor, Optional[LinearCache]]:
+        _, n = block_norm(x, next_weight=self.input_norm, eps=self.eps)
+        if hasattr(self, "linear_attn"):
+            mixed, cache = self.linear_attn(n, cache)
+        else:
+            if cache is not None:
+                raise ValueError("a softmax layer keeps no LinearCache")
+            mixed = self.self_attn(n)
+        return self._after(mixed, x), cache
+
+    def step(self, x: torch.Tensor, cache: LinearCache) -> torch.Tensor:
+        """x (batch, hidden): one token of each sequence of a linear layer."""
+        if not hasattr(self, "linear_attn"):
+            raise ValueError("only linear layers run token by token")
+        _, n = block_norm(x, next_weight=self.input_norm, eps=self.eps)
+        return self._after(self.linear_attn.step(n, cache), x)
+
+
+def run_layer(layer: nn.Module, x: torch.Tensor) -> torch.Tensor:
+    """``layer_runner`` of ``converter.convert_layer`` and
+    ``calibration.calibrate_layer`` for these layers."""
+    return layer(x)[0]

@@ -383,12 +383,12 @@ size_t exl3_delta_rule_ws_bytes(const exl3_delta_args* args);
 int exl3_delta_rule(const exl3_delta_args* args, void* ws, size_t ws_bytes, exl3_stream_t stream);
 
 /*
- * Number of CTAs of exl3_delta_rule and exl3_block_norm that gave up a bounded
- * wait for their own copies or products (2 s) since the library loaded, on the
- * current device; nonzero means that outputs of those calls are not valid.
- * Synchronizes the device.
+ * Number of CTAs of exl3_delta_rule that gave up a bounded wait for their own
+ * copies or products (2 s) since the library loaded, on the current device;
+ * nonzero means that outputs of those calls are not valid. Synchronizes the
+ * device.
  */
-int exl3_layer_fault_count(unsigned int* count);
+int exl3_delta_fault_count(unsigned int* count);
 
 /* ------------------------------------------------------------------ */
 /* Diagnostics                                                         */

@@ -13,7 +13,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from exl3_intel_arc_quantizer_b200.delta_rule import gated_delta_rule, gated_delta_step_
+from exl3_intel_arc_quantizer_b200.delta_rule import delta_fault_count, gated_delta_rule, gated_delta_step_
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -151,6 +151,25 @@ def test_zero_rows_and_large_values(dtype):
 @pytest.mark.parametrize("dtype", TYPES)
 def test_long_sequence(dtype):
     check(*inputs(1500, 1, 2, 128, 128, dtype, 10, decay=0.1), [1500], normalize_qk=True)
+    assert delta_fault_count() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_chains(dtype):
+    """More chains than the narrow slices are used for: two column groups per CTA."""
+    lens = [65, 130, 1, 64, 90, 3, 128, 70, 200, 63]
+    check(*inputs(sum(lens), 4, 16, 64, 128, dtype, 30), lens, normalize_qk=True)
+    x = inputs(200, 4, 16, 128, 192, dtype, 31)
+    state = torch.randn(8, 16, 128, 192, device=DEV, generator=torch.Generator(device=DEV).manual_seed(5))
+    check(*x, [25] * 8, state, normalize_qk=True)
+    assert delta_fault_count() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_growing_states(dtype):
+    """Positive log decays: the state grows by e^6 in the sequence."""
+    q, k, v, g, beta = inputs(300, 1, 2, 64, 64, dtype, 32)
+    check(q, k, v, g * 0 + 0.02, beta, [300], normalize_qk=True)
 
 
 def test_slices_of_one_projection_and_unaligned_ones():

@@ -157,3 +157,19 @@ def test_no_cpu_path():
                  lambda: gated_delta_step_(x, x, x, g, g, torch.zeros(1, 1, 8, 8))):
         with pytest.raises(_ext.NativeUnavailable, match="CUDA"):
             call()
+
+
+def test_hybrid_layer_names_its_projections():
+    """The Hessian groups of both kinds of layer, and what the quantizer takes."""
+    from exl3_intel_arc_quantizer_b200.calibration import hessian_groups
+    from exl3_intel_arc_quantizer_b200.hybrid import HybridDecoderLayer
+
+    layer = HybridDecoderLayer(256, 512, linear=True, key_heads=2, heads=4, key_dim=64, value_dim=64)
+    groups = hessian_groups(layer)
+    assert groups["linear_attn.input"] == ["linear_attn.in_proj_qkv", "linear_attn.in_proj_z",
+                                           "linear_attn.in_proj_b", "linear_attn.in_proj_a"]
+    assert groups["linear_attn.out_proj"] == ["linear_attn.out_proj"]
+    assert layer.quantizable() == ["linear_attn.in_proj_qkv", "linear_attn.in_proj_z", "linear_attn.out_proj",
+                                   "mlp.gate_proj", "mlp.up_proj", "mlp.down_proj"]
+    full = HybridDecoderLayer(256, 512, linear=False, heads=4, kv_heads=2, head_dim=64)
+    assert hessian_groups(full)["self_attn.input"] == ["self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj"]
