@@ -9,10 +9,15 @@
 // The second norm takes h before its rounding. Bound: HBM, each tensor moved
 // once: a row stays in registers as fp32 between its two sums. Rows of up to
 // 128 vectors belong to part of a warp or a warp (sums by shuffles), longer
-// ones to a CTA (one barrier per sum). CTAs walk over the rows and load the
-// next row's vectors before they work on this one's, so that loads are in
-// flight across the sums; rows past the registers of a CTA are read again for
-// each sum.
+// ones to a CTA (one barrier per sum); rows past the registers of a CTA are
+// read again for each sum. A thread has one vector where it can: three CTAs of
+// 512 threads then share an SM and hide one another's sums (loading the next
+// row ahead takes the registers of half of them).
+//
+// B200: 16,384 x 4,096 bf16 with both norms and the residual 105 us, 5.1 TB/s
+// (0.77 of the measured copy rate); 131,072 x 128 fp16, norm and silu gate,
+// 24.7 us, 4.1 TB/s; 3,001 x 4,095 fp16 with everything 47 us, 2.6 TB/s (rows
+// off a boundary read their parameters element by element).
 #include "common.cuh"
 #include "vec_types.cuh"
 

@@ -11,7 +11,11 @@
 // cosines and sines of its tokens in shared memory, computed once and used
 // by every head; a thread then turns 16-byte vectors (one from each half of
 // the head, or one vector of four neighbouring pairs), kUnroll of them
-// loaded before the first is turned.
+// loaded before the table is made and the first is turned.
+//
+// B200: 8 x 2,048 tokens, 32 + 8 heads of 128, fp16: 73.2 us, 4.6 TB/s (0.70 of
+// the measured copy rate); 20,001 tokens, 64 of 256 elements turned, bf16:
+// 87.4 us, 4.7 TB/s. What is left is latency at two CTAs per SM.
 #include "common.cuh"
 #include "vec_types.cuh"
 

@@ -39,7 +39,9 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     (others are copied); dk (up to 256) and dv multiples of 8. ``g`` (log
     decay, -inf allowed) and ``beta`` in float32. ``initial_state`` (sequences,
     heads, dk, dv) float32, zeros if None; the final state is a new tensor of
-    that shape. ``scale`` defaults to ``dk ** -0.5``. ``normalize_qk`` divides
+    that shape. ``scale`` defaults to ``dk ** -0.5``. Tokens are computed in
+    chunks of 64: a NaN or infinity of one token also reaches the outputs of
+    the earlier tokens of its chunk (never another sequence's). ``normalize_qk`` divides
     each q and k by ``sqrt(sum of squares + 1e-6)`` first. No autograd: with
     gradients enabled, inputs that require one are refused.
     """
