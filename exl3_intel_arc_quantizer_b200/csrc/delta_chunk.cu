@@ -234,7 +234,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // 64 KB per key head and 33 KB per head.
 template <typename T>
 __global__ void __launch_bounds__(kPrepThreads, 3)
-delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict__ ws, int vec) {
+delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict__ ws, int vec, int above) {
   extern __shared__ __align__(128) uint8_t prep_smem[];
   PrepSmem& sm = *reinterpret_cast<PrepSmem*>(prep_smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -251,6 +251,7 @@ delta_prep_kernel(const __grid_constant__ exl3_delta_args a, uint8_t* __restrict
   }
   int64_t t0, t1;
   seq_bounds(a, s, t0, t1);
+  if (t1 - t0 <= above) return;
   t0 += (slot - slot_base(t0, s)) * kChunk;
   if (t0 >= t1) return;
   const int n = (int)(t1 - t0 < kChunk ? t1 - t0 : kChunk);
@@ -742,7 +743,7 @@ __device__ __forceinline__ void fence_after() {
 template <typename T, int GROUPS, int NV, int CT>
 __global__ void __launch_bounds__(Geo<GROUPS, NV, CT>::kThreads, 1)
 delta_chain_kernel(const __grid_constant__ exl3_delta_args a, const uint8_t* __restrict__ ws,
-                   int vec) {
+                   int vec, int above) {
   using L = Geo<GROUPS, NV, CT>;
   extern __shared__ __align__(1024) uint8_t chain_smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -757,7 +758,7 @@ delta_chain_kernel(const __grid_constant__ exl3_delta_args a, const uint8_t* __r
   const int col_base = slice * GROUPS * NV;
   const int col_end = col_base + GROUPS * NV < a.dv ? col_base + GROUPS * NV : a.dv;
 
-  // tokens outside every sequence, and sequences without tokens
+  // tokens outside every sequence, then sequences without tokens
   if (s == 0 || s == a.seqs - 1) {
     const int per = (col_end - col_base) / 8;
     T* o = static_cast<T*>(a.out);
@@ -769,6 +770,7 @@ delta_chain_kernel(const __grid_constant__ exl3_delta_args a, const uint8_t* __r
           make_uint4(0, 0, 0, 0);
     }
   }
+  if (t1 - t0 <= above) return;
   if (t0 == t1) {
     const int per = (col_end - col_base) / 4;
     for (int i = tid; i < a.dk * per; i += L::kThreads) {
@@ -1187,7 +1189,7 @@ delta_chain_kernel(const __grid_constant__ exl3_delta_args a, const uint8_t* __r
 }
 
 template <typename T, int GROUPS, int NV, int CT>
-int launch_chain(const exl3_delta_args& a, const uint8_t* ws, int vec, cudaStream_t stream) {
+int launch_chain(const exl3_delta_args& a, const uint8_t* ws, int vec, int above, cudaStream_t stream) {
   using L = Geo<GROUPS, NV, CT>;
   static DeviceBits attr_done;
   int dev = 0;
@@ -1199,13 +1201,13 @@ int launch_chain(const exl3_delta_args& a, const uint8_t* ws, int vec, cudaStrea
   }
   const int64_t ctas = a.seqs * a.heads * ((a.dv + GROUPS * NV - 1) / (GROUPS * NV));
   EXL3_REQUIRE(ctas < (1ll << 31), "too many sequences and heads");
-  delta_chain_kernel<T, GROUPS, NV, CT><<<(unsigned)ctas, L::kThreads, L::kSmem, stream>>>(a, ws, vec);
+  delta_chain_kernel<T, GROUPS, NV, CT><<<(unsigned)ctas, L::kThreads, L::kSmem, stream>>>(a, ws, vec, above);
   EXL3_LAUNCHED();
   return EXL3_OK;
 }
 
 template <typename T>
-int launch_chunks(const exl3_delta_args& a, uint8_t* ws, cudaStream_t stream) {
+int launch_chunks(const exl3_delta_args& a, uint8_t* ws, int above, cudaStream_t stream) {
   static DeviceBits attr_done;
   int dev = 0;
   EXL3_CUDA(cudaGetDevice(&dev));
@@ -1222,12 +1224,12 @@ int launch_chunks(const exl3_delta_args& a, uint8_t* ws, cudaStream_t stream) {
   const int64_t slots = a.tokens / kChunk + a.seqs;
   EXL3_REQUIRE(slots < (1ll << 31) && a.key_heads < 65536, "too many tokens or heads");
   delta_prep_kernel<T><<<dim3((unsigned)slots, (unsigned)a.key_heads), kPrepThreads, sizeof(PrepSmem),
-                         stream>>>(a, ws, vec & 1);
+                         stream>>>(a, ws, vec & 1, above);
   EXL3_LAUNCHED();
   const int64_t chains = a.seqs * a.heads;
   if (chains * ((a.dv + 31) / 32) <= 2 * sm_count())
-    return launch_chain<T, 1, 32, 16>(a, ws, vec, stream);
-  return launch_chain<T, 2, 64, 32>(a, ws, vec, stream);
+    return launch_chain<T, 1, 32, 16>(a, ws, vec, above, stream);
+  return launch_chain<T, 2, 64, 32>(a, ws, vec, above, stream);
 }
 
 }  // namespace
@@ -1236,9 +1238,9 @@ size_t delta_chunk_ws_bytes(const exl3_delta_args& a) {
   return (size_t)((a.tokens / kChunk + a.seqs) * slot_bytes(a));
 }
 
-int delta_chunks(const exl3_delta_args& a, void* ws, cudaStream_t stream) {
-  return a.dtype == EXL3_F16 ? launch_chunks<__half>(a, static_cast<uint8_t*>(ws), stream)
-                             : launch_chunks<__nv_bfloat16>(a, static_cast<uint8_t*>(ws), stream);
+int delta_chunks(const exl3_delta_args& a, void* ws, int above, cudaStream_t stream) {
+  return a.dtype == EXL3_F16 ? launch_chunks<__half>(a, static_cast<uint8_t*>(ws), above, stream)
+                             : launch_chunks<__nv_bfloat16>(a, static_cast<uint8_t*>(ws), above, stream);
 }
 
 }  // namespace exl3

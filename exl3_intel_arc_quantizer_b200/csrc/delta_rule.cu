@@ -10,14 +10,17 @@
 // o, and the update follows. The norms of q and k are factors of a, b and
 // q . k and are summed by the same shuffles.
 //
-// A warp owns 4 CL columns of one head's state in registers: CL lanes hold
-// four columns each (CL = 4: a row of the slice is 64 bytes), 32 / CL lanes
-// share the rows. No two warps exchange anything. Single tokens are
-// bound by HBM: the state is read and written once (8 bytes per element).
+// A warp owns 4 CL columns of one head's state in registers (token_steps):
+// CL lanes hold four columns each (CL = 4: a row of the slice is 64 bytes),
+// 32 / CL lanes share the rows. No two warps exchange anything. Single tokens
+// are bound by HBM: the state is read and written once (8 bytes per
+// element). Longer sequences are bound by a warp's instructions, 0.5 to
+// 0.6 us per token.
 //
-// B200: 128 tokens of 32 heads of 128 x 128: 106.5 us, 5.1 TB/s (0.78 of the
-// measured copy rate) with 16 columns per warp; with 32, twice the registers
-// per thread and half the warps, 127 us.
+// B200: 128 tokens of 32 heads of 128 x 128: 93.3 us, 5.8 TB/s (0.88 of the
+// measured copy rate), 106.6 without the packed arithmetic; with
+// 32 columns per warp, twice the registers per thread and half the warps,
+// 127 us.
 #include "common.cuh"
 #include "delta_rule.cuh"
 
@@ -25,34 +28,24 @@ namespace exl3 {
 namespace {
 
 constexpr int kWarps = 4;  // per CTA
-
-// N consecutive elements from p, zero where the row of k or q ends
-template <typename T, int N>
-__device__ __forceinline__ void load_row(const T* p, int at, int d, bool vec, float (&out)[N]) {
-  if (vec) {
-#pragma unroll
-    for (int c = 0; c < N; c += 8) {
-      if (at + c < d) {  // d is a multiple of 8
-        float f[8];
-        unpack(load_raw<T, 8>(p + at + c), f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) out[c + i] = f[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) out[c + i] = 0.f;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) out[i] = at + i < d ? to_f32(p[at + i]) : 0.f;
-  }
-}
+// A pack of this many tokens is computed token by token whatever its lengths:
+// one sequence of 24 tokens takes 15.1 us, in chunks 22.5 (32 heads; 1 head
+// 14.8 and 17.9), one of 32 tokens 19.3 (1 head 18.8, where chunks win).
+constexpr int kFewTokens = 24;
+// The longest sequence that is computed token by token in a larger pack, where
+// the chains of all sequences fill the GPU more than twice or the sequences
+// are short on average: 64 sequences of 32 heads take 95 us at one token each
+// and 217 at 16, in chunks 292 and 298; at 24 tokens 270 and 300, which a
+// single one of them in a pack of long ones would lose.
+constexpr int kShort = 16;
 
 // ROWS: state rows of a thread (dk <= ROWS * 32 / CL). STEP: one token per sequence,
-// states picked by slot and written in place.
+// states picked by slot and written in place. most: the longest sequence that
+// is computed here (the chunked form has the others, and the tokens outside
+// all), or 0 for all.
 template <typename T, int ROWS, int CL, bool STEP>
 __global__ void __launch_bounds__(32 * kWarps)
-delta_tokens_kernel(const __grid_constant__ exl3_delta_args a, int vec) {
+delta_tokens_kernel(const __grid_constant__ exl3_delta_args a, int vec, int most) {
   const int lane = threadIdx.x & 31;
   constexpr int kCols = 4 * CL;
   const int slices = (a.dv + kCols - 1) / kCols;
@@ -60,18 +53,17 @@ delta_tokens_kernel(const __grid_constant__ exl3_delta_args a, int vec) {
   const int64_t sh = w / slices;
   if (sh >= a.seqs * a.heads) return;
   const int64_t s = sh / a.heads;
-  const int h = (int)(sh - s * a.heads), kh = h / (a.heads / a.key_heads);
+  const int h = (int)(sh - s * a.heads);
   const int col = (int)(w - sh * slices) * kCols + (lane % CL) * 4;
-  const int row0 = (lane / CL) * ROWS;
-  const bool in = col < a.dv;  // dv is a multiple of 8: four columns are all in or all out
+  const bool writes = col < a.dv && lane < CL;
 
-  int64_t t0, t1, from, to;
+  int64_t t0, t1, slot;
   if (STEP) {
     t0 = s;
     t1 = s + 1;
-    from = to = a.slots ? a.slots[s] : s;
-    if (from < 0 || from >= a.num_slots) {
-      if (in && lane < CL) {
+    slot = a.slots ? a.slots[s] : s;
+    if (slot < 0 || slot >= a.num_slots) {
+      if (writes) {
         T* o = static_cast<T*>(a.out) + (t0 * a.heads + h) * a.dv + col;
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[c] = from_f32<T>(0.f);
@@ -80,99 +72,53 @@ delta_tokens_kernel(const __grid_constant__ exl3_delta_args a, int vec) {
     }
   } else {
     seq_bounds(a, s, t0, t1);
-    from = to = s;
-    if (in && lane < CL) zero_outside<T>(a, s, t0, t1, h, col, 4);
+    slot = s;
+    if (most && t1 - t0 > most) return;
+    if (!most && writes) zero_outside<T>(a, s, t0, t1, h, col, 4);
   }
-  float S[ROWS][4];
-  const int64_t state_at = ((int64_t)from * a.heads + h) * a.dk * a.dv;
-#pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (a.state_in && in && row0 + i < a.dk)
-      v = *reinterpret_cast<const float4*>(a.state_in + state_at + (int64_t)(row0 + i) * a.dv + col);
-    S[i][0] = v.x;
-    S[i][1] = v.y;
-    S[i][2] = v.z;
-    S[i][3] = v.w;
-  }
-  const T* q = static_cast<const T*>(a.q) + kh * a.q_strides[1];
-  const T* k = static_cast<const T*>(a.k) + kh * a.k_strides[1];
-  const T* v = static_cast<const T*>(a.v) + h * a.v_strides[1];
-  for (int64_t t = t0; t < t1; ++t) {
-    float kr[ROWS], qr[ROWS], vr[4];
-    load_row<T, ROWS>(k + t * a.k_strides[0], row0, a.dk, vec & 1, kr);
-    load_row<T, ROWS>(q + t * a.q_strides[0], row0, a.dk, vec & 1, qr);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) vr[c] = in ? to_f32(v[t * a.v_strides[0] + col + c]) : 0.f;
-    const float G = expf(a.g[t * a.g_stride + h]), beta = a.beta[t * a.beta_stride + h];
-    // kk, qq, qk, then the four columns of S^T k and S^T q
-    float r[11];
-#pragma unroll
-    for (int j = 0; j < 11; ++j) r[j] = 0.f;
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      r[0] = fmaf(kr[i], kr[i], r[0]);
-      r[1] = fmaf(qr[i], qr[i], r[1]);
-      r[2] = fmaf(qr[i], kr[i], r[2]);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        r[3 + c] = fmaf(S[i][c], kr[i], r[3 + c]);
-        r[7 + c] = fmaf(S[i][c], qr[i], r[7 + c]);
-      }
-    }
-#pragma unroll
-    for (int o = CL; o < 32; o <<= 1)
-#pragma unroll
-      for (int j = 0; j < 11; ++j) r[j] += __shfl_xor_sync(0xFFFFFFFFu, r[j], o);
-    const float rk = a.normalize_qk ? rsqrtf(r[0] + kNormEps) : 1.f;
-    const float rq = (a.normalize_qk ? rsqrtf(r[1] + kNormEps) : 1.f) * a.scale;
-    float u[4], o[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      u[c] = beta * (vr[c] - G * rk * r[3 + c]);
-      o[c] = rq * (G * r[7 + c] + r[2] * rk * u[c]);
-    }
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      const float ki = kr[i] * rk;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) S[i][c] = fmaf(ki, u[c], G * S[i][c]);
-    }
-    if (in && lane < CL)
-      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (t * a.heads + h) * a.dv + col) =
-          make_uint2(f32_to_word<T>(make_float2(o[0], o[1])), f32_to_word<T>(make_float2(o[2], o[3])));
-  }
-  if (in)
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i)
-      if (row0 + i < a.dk)
-        *reinterpret_cast<float4*>(a.state_out + ((int64_t)to * a.heads + h) * a.dk * a.dv +
-                                   (int64_t)(row0 + i) * a.dv + col) =
-            make_float4(S[i][0], S[i][1], S[i][2], S[i][3]);
+  token_steps<T, ROWS, CL>(a, slot, h, col, t0, t1, lane, vec);
 }
 
-template <typename T, bool STEP>
-int launch_tokens(const exl3_delta_args& a, cudaStream_t stream) {
-  constexpr int kCols = 16;
+template <typename T, bool STEP, int CL>
+int launch_tokens_of(const exl3_delta_args& a, int most, cudaStream_t stream) {
+  constexpr int kCols = 4 * CL;
   const int64_t warps = a.seqs * a.heads * ((a.dv + kCols - 1) / kCols);
   const int64_t ctas = (warps + kWarps - 1) / kWarps;
   EXL3_REQUIRE(ctas < (1ll << 31), "too many sequences and heads");
   const auto fits = [](const void* p, const int64_t* st) {
     return aligned_to(p, 16) && st[0] % 8 == 0 && st[1] % 8 == 0;
   };
-  const int vec = fits(a.q, a.q_strides) && fits(a.k, a.k_strides);
+  const int vec = (fits(a.q, a.q_strides) && fits(a.k, a.k_strides) ? 1 : 0) |
+                  (aligned_to(a.v, 8) && a.v_strides[0] % 4 == 0 && a.v_strides[1] % 4 == 0 ? 2 : 0);
   if (a.dk <= 64)
-    delta_tokens_kernel<T, 8, 4, STEP><<<(unsigned)ctas, 32 * kWarps, 0, stream>>>(a, vec);
+    delta_tokens_kernel<T, 2 * CL, CL, STEP><<<(unsigned)ctas, 32 * kWarps, 0, stream>>>(a, vec, most);
   else if (a.dk <= 128)
-    delta_tokens_kernel<T, 16, 4, STEP><<<(unsigned)ctas, 32 * kWarps, 0, stream>>>(a, vec);
+    delta_tokens_kernel<T, 4 * CL, CL, STEP><<<(unsigned)ctas, 32 * kWarps, 0, stream>>>(a, vec, most);
   else
-    delta_tokens_kernel<T, 32, 4, STEP><<<(unsigned)ctas, 32 * kWarps, 0, stream>>>(a, vec);
+    delta_tokens_kernel<T, 8 * CL, CL, STEP><<<(unsigned)ctas, 32 * kWarps, 0, stream>>>(a, vec, most);
   EXL3_LAUNCHED();
   return EXL3_OK;
 }
 
-// The chunked form for all but a handful of tokens and heads too wide for it.
-bool chunked(const exl3_delta_args& a) { return a.dk <= 128 && a.tokens > 8; }
+// 16 columns per warp, or 8 while the warps of 16 would not give every
+// scheduler one: one sequence of 32 heads of 128 x 128 takes 3.0 us against 3.4
+// (one token) and 15.2 against 17.6 (24 tokens), four sequences 5.7 against 5.3
+// and 29 against 24.
+// 16 columns per warp, or 8 while the warps of 16 would not give every
+// scheduler one: one sequence of 32 heads of 128 x 128 takes 3.0 us against
+// 3.4 (one token) and 15.2 against 17.6 (24 tokens), four sequences 5.7 against
+// 5.3 and 29 against 24.
+template <bool STEP>
+int launch_tokens(const exl3_delta_args& a, int most, cudaStream_t stream) {
+  const bool few = a.seqs * a.heads * ((a.dv + 15) / 16) <= 4 * sm_count();
+  if (a.dtype == EXL3_F16)
+    return few ? launch_tokens_of<__half, STEP, 2>(a, most, stream) : launch_tokens_of<__half, STEP, 4>(a, most, stream);
+  return few ? launch_tokens_of<__nv_bfloat16, STEP, 2>(a, most, stream)
+             : launch_tokens_of<__nv_bfloat16, STEP, 4>(a, most, stream);
+}
+
+// The chunked form for all but short packs and heads too wide for it.
+bool chunked(const exl3_delta_args& a) { return a.dk <= 128 && a.tokens > kFewTokens; }
 
 int check_args(const exl3_delta_args* args) {
   EXL3_REQUIRE(args != nullptr, "args is NULL");
@@ -212,8 +158,7 @@ extern "C" int exl3_delta_step(const exl3_delta_args* args, exl3_stream_t stream
   a.state_in = a.state_out;
   if (const int rc = check_pointers(a)) return rc;
   cudaStream_t s = (cudaStream_t)stream;
-  return a.dtype == EXL3_F16 ? launch_tokens<__half, true>(a, s)
-                             : launch_tokens<__nv_bfloat16, true>(a, s);
+  return launch_tokens<true>(a, 0, s);
 }
 
 extern "C" size_t exl3_delta_rule_ws_bytes(const exl3_delta_args* args) {
@@ -234,8 +179,9 @@ extern "C" int exl3_delta_rule(const exl3_delta_args* args, void* ws, size_t ws_
   cudaStream_t s = (cudaStream_t)stream;
   if (chunked(a)) {
     EXL3_REQUIRE(aligned_to(ws, 16), "the workspace must be 16-byte aligned");
-    return delta_chunks(a, ws, s);
+    if (a.seqs * a.heads <= 2 * sm_count() && a.tokens > kShort * a.seqs) return delta_chunks(a, ws, -1, s);
+    if (const int rc = launch_tokens<false>(a, kShort, s)) return rc;
+    return delta_chunks(a, ws, kShort, s);
   }
-  return a.dtype == EXL3_F16 ? launch_tokens<__half, false>(a, s)
-                             : launch_tokens<__nv_bfloat16, false>(a, s);
+  return launch_tokens<false>(a, 0, s);
 }

@@ -294,6 +294,28 @@ def test_repeated_calls_are_bit_identical_and_streams_agree():
     assert torch.equal(o, o2) and torch.equal(S, S2)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hk,h,dk,dv", [(1, 1, 8, 8), (2, 4, 72, 40), (2, 2, 64, 192), (4, 8, 128, 128)])
+def test_short_sequences_alone_and_among_long_ones(dtype, hk, h, dk, dv):
+    lens = [1, 23, 130, 24, 0, 25, 2, 64, 16]
+    x = inputs(sum(lens), hk, h, dk, dv, dtype, 21)
+    state = torch.randn(len(lens), h, dk, dv, device=DEV, generator=torch.Generator(device=DEV).manual_seed(3)) * 0.2
+    check(*x, lens, state, normalize_qk=True)
+    for n in (9, 23, 24, 25):
+        check(*(t[:n] for t in x), [n], normalize_qk=True)
+
+
+def test_many_short_sequences_and_a_long_one():
+    lens = [1] * 90 + [300] + [7] * 60
+    x = inputs(sum(lens), 2, 4, 128, 128, torch.bfloat16, 22)
+    y = (*(torch.cat([t, t[..., :1]], -1)[..., :-1] for t in x[:3]), *x[3:])  # rows 129 elements apart
+    state = torch.randn(len(lens), 4, 128, 128, device=DEV, generator=torch.Generator(device=DEV).manual_seed(4)) * 0.2
+    check(*x, lens, state, normalize_qk=True)
+    o, S = gated_delta_rule(*x, cu_seqlens=cu_of(lens), initial_state=state, normalize_qk=True)
+    o2, S2 = gated_delta_rule(*y, cu_seqlens=cu_of(lens), initial_state=state, normalize_qk=True)
+    assert torch.equal(o, o2) and torch.equal(S, S2)
+
+
 def test_nothing_to_do():
     q, k, v, g, beta = inputs(0, 1, 2, 64, 64, torch.float16)
     o, S = gated_delta_rule(q, k, v, g, beta)
