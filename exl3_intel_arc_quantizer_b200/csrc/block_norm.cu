@@ -16,8 +16,10 @@
 //
 // B200: 16,384 x 4,096 bf16 with both norms and the residual 105 us, 5.1 TB/s
 // (0.77 of the measured copy rate); 131,072 x 128 fp16, norm and silu gate,
-// 24.7 us, 4.1 TB/s; 3,001 x 4,095 fp16 with everything 47 us, 2.6 TB/s (rows
-// off a boundary read their parameters element by element).
+// 24.7 us, 4.1 TB/s; 3,001 x 4,095 fp16 with everything 36 us, 3.4 TB/s (47 with
+// one vector per thread, whose 32 registers spilled, edges read by elements, and
+// parameters by elements for every row; 39 with parameters from two aligned
+// words shifted for every row). Rows off a boundary are bound by instructions.
 #include "common.cuh"
 #include "vec_types.cuh"
 
@@ -25,9 +27,14 @@ namespace exl3 {
 namespace {
 
 // Threads of a CTA that owns a row: three of 512 have 42 registers per thread.
-// 4,096 elements of 16 bits off a boundary are 513 vectors.
-constexpr int max_threads(bool shift) { return shift ? 544 : 512; }
+// Rows off a boundary hold two vectors per thread (4,096 elements of 16 bits
+// are 513 vectors there): three of 288 threads have 56 registers.
+constexpr int max_threads(bool shift) { return shift ? 288 : 512; }
+constexpr int max_row_threads(bool cta_row, bool shift) { return cta_row ? max_threads(shift) : 128; }
 constexpr int max_warps(bool shift) { return (max_threads(shift) / 32 + 3) / 4 * 4; }  // whole 16 bytes
+constexpr int min_ctas(int nv, bool cta_row, bool shift) {
+  return !cta_row ? (nv == 1 ? 12 : 4) : shift ? (nv == 2 ? 3 : nv == 4 ? 2 : 1) : nv == 1 ? 3 : 1;
+}
 
 __device__ __forceinline__ float act_sigmoid(float z) {
   float r;  // 2^-22; exp(-z) = inf gives 0
@@ -74,7 +81,7 @@ struct Held {
 // its elements c V - off .. c V - off + V - 1, the first and the last of them
 // moved element by element.
 template <typename T, typename P, int V, int NV, bool CTA_ROW, bool GATE, bool SHIFT>
-__global__ void __launch_bounds__(CTA_ROW ? max_threads(SHIFT) : 128, NV == 1 ? (CTA_ROW ? 3 : 12) : (CTA_ROW ? 1 : 4))
+__global__ void __launch_bounds__(max_row_threads(CTA_ROW, SHIFT), min_ctas(NV, CTA_ROW, SHIFT))
 block_norm_kernel(const __grid_constant__ exl3_block_norm_args a, int lanes) {
   constexpr int kRed = CTA_ROW ? max_warps(SHIFT) : 4;
   __shared__ __align__(16) float red[2][kRed];
@@ -102,16 +109,27 @@ block_norm_kernel(const __grid_constant__ exl3_block_norm_args a, int lanes) {
   const auto offset = [&](int64_t row) {
     return SHIFT ? (int)(reinterpret_cast<uintptr_t>(x + row * a.x_stride) / sizeof(T) % V) : 0;
   };
-  // vector c of a row that starts at p: elements e0 .. e0 + V - 1
-  const auto load = [&](const T* p, int e0) {
+  // elements e0 .. e0 + V - 1 of a row of t. A shifted row's first and last
+  // vectors are read whole, with what stands beside the row in the tensor (a
+  // branch that reads elements would wait for each tensor in turn), but for
+  // those that reach out of the tensor.
+  const auto load = [&](const T* t, int64_t stride, int64_t row, int e0) {
+    const T* const p = t + row * stride;
     if constexpr (SHIFT)
-      if (e0 < 0 || e0 + V > d) {
+      if ((e0 < 0 && (row == 0 || stride < d)) || (e0 + V > d && (row == a.rows - 1 || stride < d))) {
         float f[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) f[e] = e0 + e >= 0 && e0 + e < d ? to_f32(p[e0 + e]) : 0.f;
         return pack<T, V>(f);  // the elements' own values again
       }
     return load_piece<T, V>(p + e0);
+  };
+  // what a vector holds outside the row counts nothing
+  const auto clear_outside = [&](float (&f)[V], int e0) {
+    if (SHIFT && (e0 < 0 || e0 + V > d))
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (e0 + e < 0 || e0 + e >= d) f[e] = 0.f;
   };
   const auto store = [&](T* p, int e0, const float (&f)[V]) {
     if (!SHIFT || (e0 >= 0 && e0 + V <= d)) {
@@ -122,16 +140,35 @@ block_norm_kernel(const __grid_constant__ exl3_block_norm_args a, int lanes) {
     for (int e = 0; e < V; ++e)
       if (e0 + e >= 0 && e0 + e < d) p[e0 + e] = from_f32<T>(f[e]);
   };
-  const auto param = [&](const P* p, int e0, float (&w)[V]) {
-    if constexpr (SHIFT) {
+  // Off a boundary a thread's rows are alike (launch): its elements of the
+  // parameters are read once and kept in shared memory, aligned.
+  extern __shared__ __align__(16) uint8_t kept[];
+  const int at_next = weight ? 1 : 0, at_scale = at_next + (next_weight ? 1 : 0);
+  const auto slot = [&](int which, int i) {
+    return reinterpret_cast<P*>(kept) + ((which * NV + i) * (int)blockDim.x + (int)threadIdx.x) * V;
+  };
+  if constexpr (SHIFT) {
+    const int off = offset((int64_t)blockIdx.x * per_cta + sub);
+    const auto keep = [&](const P* p, int which) {
+      if (!p) return;
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const int at = e0 + e < 0 ? 0 : e0 + e < d ? e0 + e : d - 1;
-        w[e] = to_f32(p[at]);
+      for (int i = 0; i < NV; ++i) {
+        const int e0 = (lane + i * width) * V - off;
+        float w[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[e] = e0 + e >= 0 && e0 + e < d ? to_f32(p[e0 + e]) : 0.f;
+        store_raw<P, V>(slot(which, i), pack<P, V>(w));
       }
-    } else {
+    };
+    keep(weight, 0);
+    keep(next_weight, at_next);
+    keep(scale, at_scale);
+  }
+  const auto param = [&](const P* p, int which, int i, int e0, float (&w)[V]) {
+    if constexpr (SHIFT)
+      unpack(load_raw<P, V>(slot(which, i)), w);
+    else
       unpack(load_piece<P, V>(p + e0), w);
-    }
   };
   const int64_t step = (int64_t)gridDim.x * per_cta;
   for (int64_t r0 = (int64_t)blockIdx.x * per_cta; r0 < a.rows; r0 += step) {
@@ -148,14 +185,17 @@ block_norm_kernel(const __grid_constant__ exl3_block_norm_args a, int lanes) {
       raw.r[i] = {};
       if (GATE) raw.g[i] = {};
       if (live && e0 < d) {
-        raw.x[i] = load(x + row * a.x_stride, e0);
-        if (GATE) raw.g[i] = load(gate + row * a.gate_stride, e0);
-        if (residual) raw.r[i] = load(residual + row * a.residual_stride, e0);
+        raw.x[i] = load(x, a.x_stride, row, e0);
+        if (GATE) raw.g[i] = load(gate, a.gate_stride, row, e0);
+        if (residual) raw.r[i] = load(residual, a.residual_stride, row, e0);
       }
     }
     float y[NV][V];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) unpack(raw.x[i], y[i]);
+    for (int i = 0; i < NV; ++i) {
+      unpack(raw.x[i], y[i]);
+      clear_outside(y[i], (lane + i * width) * V - off);
+    }
     if (weight) {
       float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
@@ -166,7 +206,7 @@ block_norm_kernel(const __grid_constant__ exl3_block_norm_args a, int lanes) {
         const int e0 = (lane + i * width) * V - off;
         if (e0 >= d) break;
         float w[V];
-        param(weight, e0, w);
+        param(weight, 0, i, e0, w);
         if (a.weight_offset != 0.f) vec_add(w, a.weight_offset);
         vec_scale(y[i], r);
         vec_mul(y[i], w);
@@ -187,7 +227,7 @@ block_norm_kernel(const __grid_constant__ exl3_block_norm_args a, int lanes) {
         unpack(raw.r[i], res);
         if (scale) {
           float w[V];
-          param(scale, e0, w);
+          param(scale, at_scale, i, e0, w);
           vec_scale(w, a.residual_scale);
           vec_fma(y[i], w, res);
         } else {
@@ -201,11 +241,7 @@ block_norm_kernel(const __grid_constant__ exl3_block_norm_args a, int lanes) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int e0 = (lane + i * width) * V - off;
-        // what a vector holds outside the row counts nothing
-        if (SHIFT && (e0 < 0 || e0 + V > d))
-#pragma unroll
-          for (int e = 0; e < V; ++e)
-            if (e0 + e < 0 || e0 + e >= d) y[i][e] = 0.f;
+        clear_outside(y[i], e0);
         if (e0 < d) vec_squares(y[i], ss);
       }
       const float r = rsqrtf(row_sum<CTA_ROW>(ss.x + ss.y, lanes, red, side) * inv_d + a.eps);
@@ -214,7 +250,7 @@ block_norm_kernel(const __grid_constant__ exl3_block_norm_args a, int lanes) {
         const int e0 = (lane + i * width) * V - off;
         if (e0 >= d) break;
         float w[V];
-        param(next_weight, e0, w);
+        param(next_weight, at_next, i, e0, w);
         if (a.weight_offset != 0.f) vec_add(w, a.weight_offset);
         vec_scale(y[i], r);
         vec_mul(w, y[i]);
@@ -283,16 +319,31 @@ int launch(const exl3_block_norm_args& a, int threads, int lanes, cudaStream_t s
   const auto kernel = block_norm_kernel<T, P, V, NV, CTA_ROW, GATE, SHIFT>;
   const int per_cta = CTA_ROW ? 1 : threads / lanes;
   const int64_t ctas = (a.rows + per_cta - 1) / per_cta;
-  // as many CTAs as run at once: each has a next row to load
-  static std::atomic<int> known[max_threads(true) / 32 + 1];  // by warps of a CTA
-  int resident = known[threads / 32].load(std::memory_order_relaxed);
-  if (resident == 0) {
-    EXL3_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, threads, 0));
-    if (resident < 1) resident = 1;
-    known[threads / 32].store(resident, std::memory_order_relaxed);
+  const int params = (a.weight ? 1 : 0) + (a.next_weight ? 1 : 0) + (a.scale ? 1 : 0);
+  const size_t smem = SHIFT ? (size_t)params * NV * threads * V * sizeof(P) : 0;
+  if (SHIFT) {
+    static DeviceBits attr_done;
+    int dev = 0;
+    EXL3_CUDA(cudaGetDevice(&dev));
+    if (!attr_done.has(dev)) {
+      EXL3_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)(3 * NV * max_row_threads(CTA_ROW, SHIFT) * V * sizeof(P))));
+      attr_done.set(dev);
+    }
   }
-  const int64_t most = (int64_t)sm_count() * resident;
-  kernel<<<(unsigned)(ctas < most ? ctas : most), threads, 0, stream>>>(a, lanes);
+  // as many CTAs as run at once: each has a next row to load
+  static std::atomic<int> known[max_threads(false) / 32 + 1][4];  // by warps of a CTA and parameters
+  std::atomic<int>& entry = known[threads / 32][SHIFT ? params : 0];
+  int resident = entry.load(std::memory_order_relaxed);
+  if (resident == 0) {
+    EXL3_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, threads, smem));
+    if (resident < 1) resident = 1;
+    entry.store(resident, std::memory_order_relaxed);
+  }
+  int64_t most = (int64_t)sm_count() * resident;
+  // every V-th row is as far past a boundary as the first
+  if (SHIFT && ctas > most) most = most / V * V;
+  kernel<<<(unsigned)(ctas < most ? ctas : most), threads, smem, stream>>>(a, lanes);
   EXL3_LAUNCHED();
   return EXL3_OK;
 }
@@ -309,10 +360,13 @@ int launch_v(const exl3_block_norm_args& a, cudaStream_t stream) {
     return launch<T, P, V, 4, false, GATE, SHIFT>(a, 128, lanes, stream);
   }
   const auto threads = [&](int nv) { return (int)((nvec + 32 * nv - 1) / (32 * nv)) * 32; };
-  if (nvec <= max_threads(SHIFT))
-    return launch<T, P, V, 1, true, GATE, SHIFT>(a, threads(1), 32, stream);
-  if (nvec <= 2 * max_threads(SHIFT)) return launch<T, P, V, 2, true, GATE, SHIFT>(a, threads(2), 32, stream);
-  if (nvec <= 4 * max_threads(SHIFT)) return launch<T, P, V, 4, true, GATE, SHIFT>(a, threads(4), 32, stream);
+  constexpr int kFirst = SHIFT ? 2 : 1;
+  if (nvec <= kFirst * max_threads(SHIFT))
+    return launch<T, P, V, kFirst, true, GATE, SHIFT>(a, threads(kFirst), 32, stream);
+  if (nvec <= 2 * kFirst * max_threads(SHIFT))
+    return launch<T, P, V, 2 * kFirst, true, GATE, SHIFT>(a, threads(2 * kFirst), 32, stream);
+  if (nvec <= 4 * kFirst * max_threads(SHIFT))
+    return launch<T, P, V, 4 * kFirst, true, GATE, SHIFT>(a, threads(4 * kFirst), 32, stream);
   const int64_t most = (int64_t)sm_count() * 2;
   block_norm_long_kernel<T, P>
       <<<(unsigned)(a.rows < most ? a.rows : most), 1024, 0, stream>>>(a);

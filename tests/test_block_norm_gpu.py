@@ -206,3 +206,23 @@ def test_many_strided_rows():
     run_and_check(x, dict(weight=w, residual=res.contiguous()))
     wide = rand((900, 4096 + 64), torch.float16, 3)
     run_and_check(wide[:, :4096], dict(residual=wide[:, 64:], next_weight=rand(4096, torch.float32, 4)))
+
+
+@pytest.mark.parametrize("dtype,param", [(torch.float16, torch.float16), (torch.bfloat16, torch.float32),
+                                         (torch.float32, torch.float32)])
+@pytest.mark.parametrize("rows,d", [(1, 333), (3, 1001), (900, 77), (700, 4095), (460, 4610), (300, 9001), (9, 18003)])
+def test_rows_off_a_boundary(dtype, param, rows, d):
+    """What stands beside a row is not part of it, and every length keeps its own parameters."""
+    x, kw = inputs(rows, d, dtype, param, "wGrsn")
+    want = run_and_check(x, kw)
+    beside = torch.full((rows, d + 8), float("nan"), dtype=dtype, device=DEV)[:, :d]
+    beside.copy_(x)
+    got = block_norm(beside, **kw)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_overlapping_rows_off_a_boundary():
+    d = 1001
+    x = rand(40 * d, torch.float16, 1).as_strided((37, d), (d - 8, 1))
+    _, kw = inputs(37, d, torch.float16, torch.float16, "wrn")
+    run_and_check(x, kw)
