@@ -226,3 +226,8 @@ def test_overlapping_rows_off_a_boundary():
     x = rand(40 * d, torch.float16, 1).as_strided((37, d), (d - 8, 1))
     _, kw = inputs(37, d, torch.float16, torch.float16, "wrn")
     run_and_check(x, kw)
+
+
+@pytest.mark.parametrize("d", [16, 128, 77, 250])
+def test_many_short_rows(d):
+    run_and_check(*inputs(160_000 if d < 100 else 40_000, d, torch.float16, torch.float16, "wgrn"))
