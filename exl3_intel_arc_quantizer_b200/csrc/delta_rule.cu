@@ -17,7 +17,7 @@
 // element). Longer sequences are bound by a warp's instructions, 0.5 to
 // 0.6 us per token.
 //
-// B200: 128 tokens of 32 heads of 128 x 128: 93.3 us, 5.8 TB/s (0.88 of the
+// B200: 128 tokens of 32 heads of 128 x 128: 93 to 98 us, 5.6 TB/s (0.86 of the
 // measured copy rate), 106.6 without the packed arithmetic; with
 // 32 columns per warp, twice the registers per thread and half the warps,
 // 127 us.
